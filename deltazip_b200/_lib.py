@@ -119,6 +119,17 @@ class LightningArgs(Structure):
     ]
 
 
+class SharedAttentionArgs(Structure):
+    """Mirror of dz_shared_attention_args."""
+    _fields_ = [
+        ("qkv", c_void_p), ("q_row_stride", c_int64), ("out", c_void_p), ("k_cache", c_void_p), ("v_cache", c_void_p),
+        ("cache_rows", c_int64), ("block_tables", c_void_p), ("table_width", c_int32), ("block_size", c_int32),
+        ("seq_lens", c_void_p), ("group_starts", c_void_p), ("shared_lens", c_void_p), ("num_groups", c_int32),
+        ("num_seqs", c_int32), ("max_group", c_int32), ("max_shared", c_int32), ("q_heads", c_int32), ("kv_heads", c_int32),
+        ("head_dim", c_int32), ("scale", c_float), ("workspace", c_void_p), ("workspace_bytes", c_size_t), ("dtype", c_int32),
+    ]
+
+
 class DeltaZipError(RuntimeError):
     def __init__(self, status: int, where: str, detail: str = ""):
         self.status = status
@@ -201,6 +212,13 @@ _SIGNATURES = {
     "dz_moe_gather": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_int, c_void_p]),
     "dz_moe_gemm": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,
                             c_int, c_void_p, c_void_p]),
+    "dz_beam_select_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "dz_beam_select": (c_int, [c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p,
+                               c_void_p, c_size_t, c_int, c_void_p]),
+    "dz_copy_pages_max_pairs": (c_int, []),
+    "dz_copy_pages": (c_int, [c_void_p, c_int, c_int, c_int, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
+    "dz_shared_attention_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "dz_shared_attention_decode": (c_int, [POINTER(SharedAttentionArgs), c_void_p]),
     "dz_slot_upload": (c_int, [c_void_p, c_void_p, c_size_t, c_int, c_void_p]),
     "dz_slot_reset": (c_int, [c_void_p, c_size_t, c_void_p]),
     "dz_stream_fence": (c_int, [c_void_p]),

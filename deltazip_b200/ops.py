@@ -993,6 +993,142 @@ def mlstm(x: torch.Tensor, h: torch.Tensor, w_if: torch.Tensor, b_if: torch.Tens
 
 
 # ---------------------------------------------------------------------------
+# beam search over the caches
+# ---------------------------------------------------------------------------
+
+def _need_here(*tensors) -> None:
+    """CUDA tensors of the current device, on whose stream the work is enqueued."""
+    _need_cuda(*tensors)
+    here = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t is not None and t.device.index != here:
+            raise ValueError(f"a tensor is on GPU {t.device.index}, the current one is {here}")
+
+
+def _need_int32(what: str, *tensors) -> None:
+    if any(t is not None and (t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous()) for t in tensors):
+        raise ValueError(f"{what} must be contiguous int32 vectors")
+
+
+class BeamCandidates(NamedTuple):
+    """The best continuations of every group, [groups, k], best first."""
+    scores: torch.Tensor                # float32, -inf where a group has no further candidate
+    rows: torch.Tensor                  # int32, the row that is continued, -1: none
+    tokens: torch.Tensor                # int32, by which token
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, group_starts: torch.Tensor, k: int) -> BeamCandidates:
+    """The k best of scores[r] + log softmax(logits)[r, v] over the rows of every group and all tokens (dz_beam_select).
+    `logits` [rows, vocab] in 16 or 32 bits with unit column stride, `scores` [rows] float32 (the rows' cumulative
+    log-probabilities, -inf for a row that is not continued), group g being rows group_starts[g] ... group_starts[g + 1] - 1
+    (int32, rising).  Ties go to the lower row, then the lower token.  Nothing synchronises with the host."""
+    _need_here(logits, scores, group_starts)
+    _need_int32("group_starts", group_starts)
+    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError("logits must be [rows, vocab] with unit column stride")
+    rows, vocab = logits.shape
+    if scores.shape != (rows,) or scores.dtype != torch.float32 or not scores.is_contiguous():
+        raise ValueError("scores must be a contiguous float32 vector with one entry per row")
+    if group_starts.numel() < 1:
+        raise ValueError("group_starts holds the first row of every group and the end")
+    code, groups, k = _any_dtype_code(logits), group_starts.numel() - 1, int(k)
+    stride = logits.stride(0) if rows > 1 else vocab
+    out = torch.empty((3, groups, max(k, 0)), dtype=torch.int32, device=logits.device)
+    # fresh scratch for every call: two captured graphs never share it
+    ws = torch.empty(lib().dz_beam_select_workspace_bytes(rows, vocab, k), dtype=torch.uint8, device=logits.device)
+    check(lib().dz_beam_select(logits.data_ptr(), stride, rows, vocab, scores.data_ptr(), group_starts.data_ptr(), groups, k,
+                               out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), ws.data_ptr(), ws.numel(), code,
+                               _stream()), "dz_beam_select")
+    return BeamCandidates(out[0].view(torch.float32), out[1], out[2])
+
+
+class PagePools:
+    """The pools whose pages `copy_pages` copies between: tensors of [pages * rows_per_page, ...] (contiguous, any type),
+    page i being rows i * rows_per_page ... of each.  Pools of recurrent states have one row a page, a sequence's slot."""
+
+    def __init__(self, tensors, rows_per_page: int = 1):
+        tensors = list(tensors)
+        _need_here(*tensors)
+        self.rows_per_page = int(rows_per_page)
+        if self.rows_per_page < 1 or any(t.dim() < 1 or not t.is_contiguous() or t.shape[0] % self.rows_per_page for t in tensors):
+            raise ValueError("pools are contiguous tensors of whole pages")
+        counts = {t.shape[0] // self.rows_per_page for t in tensors}
+        if len(counts) > 1:
+            raise ValueError("all pools have the same number of pages")
+        self.num_pages = counts.pop() if counts else 0
+        self.tensors = [t for t in tensors if t.numel()]        # kept: the table holds their addresses
+        if len({t.device for t in self.tensors}) > 1:
+            raise ValueError("all pools are on one GPU")
+        entries, self.page_units = [], 0
+        for t in self.tensors:
+            row = t.numel() // t.shape[0] * t.element_size()
+            unit = next(u for u in (16, 8, 4, 2, 1) if row % u == 0 and t.data_ptr() % u == 0)
+            entries.append([t.data_ptr(), row, self.rows_per_page, unit])
+            self.page_units += row // unit * self.rows_per_page
+        self.device = self.tensors[0].device if self.tensors else None
+        self.table = torch.tensor(entries, dtype=torch.int64).to(self.device) if entries else None
+
+
+def copy_pages(pools: PagePools, src: torch.Tensor, dst: torch.Tensor, rows: Optional[torch.Tensor] = None) -> None:
+    """Page dst[i] of every pool becomes what page src[i] was before the call -- its first rows[i] rows where `rows` is
+    given -- for all i at once: a page may be source and destination (dz_copy_pages).  int32 vectors of at most
+    `copy_pages_max_pairs()` entries; pairs with a page outside the pools are left out, of several with one destination
+    the last counts.  Nothing synchronises with the host."""
+    _need_here(src, dst, rows)
+    _need_int32("src / dst / rows", src, dst, rows)
+    if src.shape != dst.shape or (rows is not None and rows.shape != src.shape):
+        raise ValueError("src, dst and rows have one entry per pair")
+    if pools.table is None:
+        return
+    _need_here(pools.table)
+    check(lib().dz_copy_pages(pools.table.data_ptr(), len(pools.tensors), pools.num_pages, pools.rows_per_page, pools.page_units,
+                              src.data_ptr(), dst.data_ptr(), _ptr(rows), src.numel(), _stream()), "dz_copy_pages")
+
+
+def copy_pages_max_pairs() -> int:
+    return lib().dz_copy_pages_max_pairs()
+
+
+def shared_attention_decode(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                            seq_lens: torch.Tensor, group_starts: torch.Tensor, shared_lens: torch.Tensor, max_group: int,
+                            max_shared: int, q_heads: int, kv_heads: int, block_size: int, scale: float,
+                            out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """paged_attention_decode for sequences that share their first pages: the sequences group_starts[g] ...
+    group_starts[g + 1] - 1 have their first shared_lens[g] tokens in the same cache rows, which are read once for all of
+    them (dz_shared_attention_decode).  `max_group`, `max_shared`: the most sequences of a group and the longest shared
+    length; beyond them a sequence, or what is longer, is read by itself.  Returns [B, q_heads*128]."""
+    _need_here(qkv, k_cache, v_cache, block_tables, seq_lens, group_starts, shared_lens, out)
+    _need_int32("seq_lens / group_starts / shared_lens", seq_lens, group_starts, shared_lens)
+    b, width = qkv.shape[0], (q_heads + 2 * kv_heads) * 128
+    if qkv.dim() != 2 or qkv.shape[1] < q_heads * 128 or (qkv.stride(1) != 1 and b):
+        raise ValueError(f"qkv must be [B, {width}] rows with unit column stride")
+    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 or not block_tables.is_contiguous() or \
+            block_tables.shape[0] != b or seq_lens.numel() != b:
+        raise ValueError("block_tables [B, pages] and seq_lens [B] must be contiguous int32")
+    if shared_lens.numel() != max(0, group_starts.numel() - 1):
+        raise ValueError("group_starts has one entry more than shared_lens")
+    for cache in (k_cache, v_cache):
+        if cache.dim() != 3 or tuple(cache.shape[1:]) != (kv_heads, 128) or cache.dtype != qkv.dtype or not cache.is_contiguous():
+            raise ValueError(f"the caches must be contiguous [slots, {kv_heads}, 128] of the queries' type")
+    if k_cache.shape != v_cache.shape:
+        raise ValueError("the caches of keys and values have the same slots")
+    if out is None:
+        out = torch.empty((b, q_heads * 128), dtype=qkv.dtype, device=qkv.device)
+    elif out.shape != (b, q_heads * 128) or out.dtype != qkv.dtype or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous [{b}, {q_heads * 128}] of the queries' type")
+    groups, keys = shared_lens.numel(), block_tables.shape[1] * block_size
+    ws = torch.empty(lib().dz_shared_attention_workspace_bytes(b, groups, max_group, max_shared, keys, q_heads, kv_heads),
+                     dtype=torch.uint8, device=qkv.device)
+    args = _lib.SharedAttentionArgs(
+        qkv.data_ptr(), qkv.stride(0) if b > 1 else width, out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0],
+        block_tables.data_ptr(), block_tables.shape[1], block_size, seq_lens.data_ptr(), group_starts.data_ptr(),
+        shared_lens.data_ptr(), groups, b, max_group, max_shared, q_heads, kv_heads, 128, float(scale), ws.data_ptr(), ws.numel(),
+        _dtype_code(qkv))
+    check(lib().dz_shared_attention_decode(ctypes.byref(args), _stream()), "dz_shared_attention_decode")
+    return out
+
+
+# ---------------------------------------------------------------------------
 # routed experts
 # ---------------------------------------------------------------------------
 

@@ -551,6 +551,60 @@ int dz_moe_gemm(const void* x, const void* weights, const int32_t* offsets, cons
                 int K, int experts, int act, int typical, int dtype, int* status, void* stream);
 
 /*
+ * Beam search over the caches: selection, copies of pages and states, attention over shared pages.
+ *
+ *   beam_select   logits z [rows, vocab] (dtype, rows row_stride elements apart), scores c [rows]; group g holds
+ *                 rows group_starts[g] <= r < group_starts[g + 1] (rising) and gets the k best continuations by
+ *                 c[r] + z[r, v] - log sum_v exp z[r, v], best first, ties to the lower row, then the lower token.
+ *                 NaN logits count as -inf; logits of +inf share the whole probability of their row (the order of
+ *                 the others is not said); rows without a logit above -inf or with a score that is not finite have
+ *                 scores of -inf alone.  Places without a candidate: score -inf, row and token -1.  k <= 128,
+ *                 rows <= 65535.  The workspace needs no preparation.
+ *   copy_pages    pools: a device table of num_pools entries {address, bytes of a row, rows of a page, bytes of a unit},
+ *                 a unit being the largest power of two up to 16 that divides address and row bytes; a pool is num_pages
+ *                 pages of page_rows rows.  For pairs (src, dst, rows) the first rows (NULL: all) of page dst become
+ *                 what those of page src were before the call, in every pool.  A page may be source and destination;
+ *                 of several pairs with one destination the last counts; pairs with a page outside [0, num_pages) are
+ *                 left out.  page_units: units of a page in all pools together.  At most dz_copy_pages_max_pairs() pairs.
+ *   shared_attention_decode
+ *                 dz_paged_attention_decode for sequences in groups: sequences group_starts[g] <= s <
+ *                 group_starts[g + 1] (rising) have their first shared_lens[g] tokens in the same cache rows (their
+ *                 tables begin alike), which are read once for the first max_group of them.  A sequence shorter than
+ *                 that, or outside the groups, is read by itself; shared lengths above max_shared are read as
+ *                 max_shared.  1 to 16 query heads per kv head.  A page number outside the cache is read as the
+ *                 nearest row of it.  The workspace (dz_shared_attention_workspace_bytes, max_keys = table_width *
+ *                 block_size) needs no preparation.
+ */
+size_t dz_beam_select_workspace_bytes(int rows, int vocab, int k);
+int dz_beam_select(const void* logits, int64_t row_stride, int rows, int vocab, const float* scores, const int32_t* group_starts,
+                   int num_groups, int k, float* out_scores, int32_t* out_rows, int32_t* out_tokens, void* workspace,
+                   size_t workspace_bytes, int dtype, void* stream);
+int dz_copy_pages_max_pairs(void);
+int dz_copy_pages(const int64_t* pools, int num_pools, int num_pages, int page_rows, int64_t page_units, const int32_t* src,
+                  const int32_t* dst, const int32_t* rows, int pairs, void* stream);
+typedef struct dz_shared_attention_args {
+  const void* qkv;
+  int64_t q_row_stride;
+  void* out;                /* [num_seqs, q_heads * 128] */
+  const void* k_cache;      /* [cache_rows, kv_heads, 128] */
+  const void* v_cache;
+  int64_t cache_rows;
+  const int32_t* block_tables;
+  int32_t table_width, block_size;
+  const int32_t* seq_lens;
+  const int32_t* group_starts;
+  const int32_t* shared_lens;
+  int32_t num_groups, num_seqs, max_group, max_shared, q_heads, kv_heads, head_dim;
+  float scale;
+  void* workspace;
+  size_t workspace_bytes;
+  int32_t dtype;
+} dz_shared_attention_args;
+size_t dz_shared_attention_workspace_bytes(int num_seqs, int num_groups, int max_group, int max_shared, int max_keys, int q_heads,
+                                           int kv_heads);
+int dz_shared_attention_decode(const dz_shared_attention_args* args, void* stream);
+
+/*
  * Delta swap-in: one asynchronous host->device copy of a delta's slot bytes
  * from PINNED host memory on `copy_stream`, preceded by a zero fill of the
  * destination when `zero_first` != 0 (the reference resets a slot before it
