@@ -9,6 +9,25 @@ from typing import List, Optional, Sequence, Tuple
 
 import torch
 
+from . import ops
+
+
+def _copy(handle: "ops.PagePools", device, src: Sequence[int], dst: Sequence[int], rows: Optional[Sequence[int]] = None) -> None:
+    """copy_pages of pages given as numbers on the host; more than a launch takes go in several (none of them is then both
+    source and destination)."""
+    if not src or handle.table is None:
+        return
+    most = ops.copy_pages_max_pairs()
+    index = torch.tensor([list(src), list(dst)] + ([list(rows)] if rows is not None else []), dtype=torch.int32).to(device)
+    for i in range(0, len(src), most):
+        part = [t[i:i + most] for t in index]
+        ops.copy_pages(handle, part[0], part[1], part[2] if rows is not None else None)
+
+
+def _check_pages(what: str, pages: Sequence[int], count: int, distinct: bool = False) -> None:
+    if any(not 0 <= p < count for p in pages) or (distinct and len(set(pages)) != len(pages)):
+        raise ValueError(f"{what} are {'different ' if distinct else ''}numbers from 0 to {count - 1}")
+
 
 class RecurrentStateCache:
     """Per recurrent layer run the 32-bit pools S [slots, heads, dim, vdim] and, where the run normalises
@@ -24,6 +43,8 @@ class RecurrentStateCache:
         self.n = [torch.zeros((slots, h, d), **f32) if w else None for (h, d, _), w in zip(shapes, with_n)]
         self.m = [torch.zeros((slots, h), **f32) if w else None for (h, _, _), w in zip(shapes, with_n)]
         self.free: List[int] = list(range(slots - 1, -1, -1))
+        self.slots, self.device = slots, device
+        self._pools: Optional[ops.PagePools] = None
 
     def allocate(self) -> int:
         if not self.free:
@@ -32,6 +53,26 @@ class RecurrentStateCache:
 
     def release(self, slot: int) -> None:
         self.free.append(slot)
+
+    def copy(self, src: Sequence[int], dst: Sequence[int]) -> None:
+        """The states in slots `dst` become those that slots `src` held before, in every run, all at once."""
+        _check_pages("slots", src, self.slots)
+        _check_pages("slots that are written", dst, self.slots, distinct=True)
+        if len(src) != len(dst):
+            raise ValueError("a source for every destination")
+        if self._pools is None:
+            self._pools = ops.PagePools([t for t in self.S + self.n + self.m if t is not None])
+        if len(src) > ops.copy_pages_max_pairs() and set(src) & set(dst):
+            raise ValueError(f"at most {ops.copy_pages_max_pairs()} slots that follow one another at once")
+        _copy(self._pools, self.device, src, dst)
+
+    def reorder(self, slots: Sequence[int], parents: Sequence[int]) -> None:
+        """Sequence i of those in `slots` goes on from the state of sequence parents[i] (a number among them)."""
+        _check_pages("parents", parents, len(slots))
+        if len(slots) != len(parents):
+            raise ValueError("a parent for every slot")
+        moved = [(slots[p], s) for s, p in zip(slots, parents) if slots[p] != s]
+        self.copy([a for a, _ in moved], [b for _, b in moved])
 
 
 class PagedKVCache:
@@ -43,7 +84,10 @@ class PagedKVCache:
     `window`: the largest number of tokens any layer looks back (itself included).  A sequence then
     owns at most ceil(window / block_size) blocks and uses them as a ring: token position t lives in
     block number (t / block_size) modulo the blocks it owns.  `state` holds the recurrent layers'
-    slots, where the model has any."""
+    slots, where the model has any.
+
+    Sequences may share blocks (`fork`).  A block goes back to the free list when the last of them gives it up, and `own`
+    gives a sequence a copy of a shared block before it writes to it."""
 
     def __init__(self, num_layers: int, num_blocks: int, kv_heads: int, block_size: int = 16,
                  dtype=torch.float16, device="cuda",
@@ -57,6 +101,10 @@ class PagedKVCache:
         self.window = window
         self.state = state
         self.free: List[int] = list(range(num_blocks - 1, -1, -1))
+        self.device = device
+        self.holders: List[int] = [0] * num_blocks              # sequences that hold a block
+        self.shared = 0                                         # holders beyond the first, over all blocks
+        self._pools: Optional[ops.PagePools] = None
 
     def blocks_for(self, tokens: int) -> int:
         """Blocks a sequence of `tokens` tokens holds at most."""
@@ -67,10 +115,21 @@ class PagedKVCache:
     def allocate(self, n_blocks: int) -> List[int]:
         if n_blocks > len(self.free):
             raise RuntimeError("out of KV cache blocks")
-        return [self.free.pop() for _ in range(n_blocks)]
+        blocks = [self.free.pop() for _ in range(n_blocks)]
+        for b in blocks:
+            self.holders[b] = 1
+        return blocks
 
     def release(self, blocks: Sequence[int]) -> None:
-        self.free.extend(blocks)
+        """Gives up one holder's claim on each of `blocks`."""
+        for b in blocks:
+            if self.holders[b] < 1:
+                raise RuntimeError(f"cache block {b} is not in use")
+            self.holders[b] -= 1
+            if self.holders[b]:
+                self.shared -= 1
+            else:
+                self.free.append(b)
 
     def slots(self, blocks: Sequence[int], start: int, count: int) -> List[int]:
         """Cache slots of token positions [start, start + count) of a sequence owning `blocks`.  Where
@@ -105,6 +164,90 @@ class PagedKVCache:
             self.state.release(seq.state_slot)
             seq.state_slot = -1
 
+    # -- shared blocks -----------------------------------------------------------------
+    def fork(self, pairs: Sequence[Tuple[object, object]]) -> None:
+        """For (parent, child) pairs the child goes on from what the parent has in the cache: it holds the same blocks and,
+        with recurrent layers, a copy of the state in a slot of its own (one launch for all pairs)."""
+        if self.state is not None and len(pairs) > len(self.state.free):
+            raise RuntimeError("out of recurrent state slots")
+        for parent, child in pairs:
+            child.blocks = list(parent.blocks)
+            for b in child.blocks:
+                self.holders[b] += 1
+            self.shared += len(child.blocks)
+            if self.state is not None:
+                child.state_slot = self.state.allocate()
+        if self.state is not None:
+            self.state.copy([p.state_slot for p, _ in pairs], [c.state_slot for _, c in pairs])
+
+    def own(self, work: Sequence[Tuple[object, int]]) -> bool:
+        """Before (sequence, count) write `count` tokens from position sequence.length on: the blocks these go to become the
+        sequence's own, a shared one as a copy of what it holds of the tokens before (one launch for all).  Returns whether
+        any sequence's blocks changed."""
+        if not self.shared:
+            return False
+        bs, todo = self.block_size, []
+        for seq, count in work:
+            seen = set()
+            for at in range(seq.length // bs, (seq.length + count - 1) // bs + 1 if count > 0 else 0):
+                # a ring's block still holds tokens of the last round behind the one that is written
+                i, rows = (at, max(0, seq.length - at * bs)) if self.window is None else (at % len(seq.blocks), bs)
+                if self.holders[seq.blocks[i]] > 1 and i not in seen:
+                    seen.add(i)
+                    todo.append((seq, i, rows))
+        left, new = {}, []
+        for seq, i, _ in todo:                                  # who comes last keeps the block
+            b = seq.blocks[i]
+            left[b] = left.get(b, self.holders[b]) - 1
+            new.append(left[b] > 0)
+        if sum(new) > len(self.free):
+            raise RuntimeError("out of KV cache blocks")
+        src, dst, kept = [], [], []
+        for (seq, i, rows), fresh in zip(todo, new):
+            if not fresh:
+                continue
+            (b,) = self.allocate(1)
+            if rows:
+                src.append(seq.blocks[i])
+                dst.append(b)
+                kept.append(rows)
+            self.release([seq.blocks[i]])
+            seq.blocks = seq.blocks[:i] + [b] + seq.blocks[i + 1:]
+        self.copy(src, dst, kept)
+        return any(new)
+
+    def copy(self, src: Sequence[int], dst: Sequence[int], rows: Optional[Sequence[int]] = None) -> None:
+        """Copies the first `rows` tokens (default: all) of blocks `src` to blocks `dst` in every run; no block is both."""
+        _check_pages("blocks", src, self.num_blocks)
+        _check_pages("blocks that are written", dst, self.num_blocks, distinct=True)
+        if len(src) != len(dst) or (rows is not None and len(rows) != len(src)) or set(src) & set(dst):
+            raise ValueError("a source for every destination, and none of them a destination")
+        if not src or not any(t.numel() for t in self.k + self.v):
+            return
+        if self._pools is None:
+            self._pools = ops.PagePools(self.k + self.v, self.block_size)
+        _copy(self._pools, self.device, src, dst, rows)
+
+    def compact(self, seqs: Sequence[object]) -> int:
+        """Moves the blocks in use to the lowest numbers, so that all behind them are free; `seqs`: every sequence that
+        holds any.  Returns how many there are."""
+        held: dict = {}
+        for seq in seqs:
+            for b in seq.blocks:
+                held[b] = held.get(b, 0) + 1
+        if any(held.get(b, 0) != n for b, n in enumerate(self.holders)):
+            raise ValueError("all sequences that hold blocks have to be given")
+        used = len(held)
+        high = sorted(b for b in held if b >= used)
+        move = dict(zip(high, (b for b in range(used) if b not in held)))
+        self.copy(list(move), list(move.values()))
+        for a, b in move.items():
+            self.holders[b], self.holders[a] = self.holders[a], 0
+        for seq in seqs:
+            seq.blocks = [move.get(b, b) for b in seq.blocks]
+        self.free = list(range(self.num_blocks - 1, used - 1, -1))
+        return used
+
 
 @dataclass
 class AttnMeta:
@@ -117,7 +260,10 @@ class AttnMeta:
     Models that continue prompts from a cache also read `q_starts` [B + 1] int32 (first row of every
     sequence), `ctx_lens` [B] int32 (tokens before the first row; `host_ctx_lens` the same as numbers, for
     prompt portions) and, with recurrent layers, `state_slots` [B] int32.  `shared` keeps what the layers
-    of one pass derive from all this."""
+    of one pass derive from all this.
+
+    Where sequences share cache blocks, a decode step may say so: sequences group_starts[g] ... group_starts[g + 1] - 1
+    have their first shared_lens[g] tokens in common, `max_group` and `max_shared` being the largest of both."""
     slot_mapping: Optional[torch.Tensor] = None          # int64 [M] cache slot per token, -1 = none
     block_tables: Optional[torch.Tensor] = None
     seq_lens: Optional[torch.Tensor] = None
@@ -129,6 +275,10 @@ class AttnMeta:
     host_ctx_lens: Optional[List[int]] = None
     positions: Optional[torch.Tensor] = None             # int64 [M], set by models whose mixers read them
     shared: dict = field(default_factory=dict)
+    group_starts: Optional[torch.Tensor] = None          # int32 [G + 1]
+    shared_lens: Optional[torch.Tensor] = None           # int32 [G]
+    max_group: int = 0
+    max_shared: int = 0
 
     @property
     def decode(self) -> bool:

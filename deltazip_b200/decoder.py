@@ -104,5 +104,9 @@ class LayeredDecoder(nn.Module):
     def logits(self, hidden: torch.Tensor) -> torch.Tensor:
         raise NotImplementedError
 
+    def beam_logits(self, hidden: torch.Tensor) -> torch.Tensor:
+        """What a beam search selects from, over the whole vocabulary."""
+        return self.logits(hidden)
+
     def greedy_tokens(self, hidden: torch.Tensor) -> torch.Tensor:
         return self.logits(hidden).argmax(dim=-1)

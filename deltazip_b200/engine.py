@@ -8,11 +8,11 @@ model, sample) -- reduced to greedy sampling and to what the throughput configur
 from __future__ import annotations
 
 from dataclasses import dataclass, field
-from typing import Dict, List, Optional, Tuple
+from typing import Dict, List, NamedTuple, Optional, Tuple
 
 import torch
 
-from . import registry
+from . import ops, registry
 from .cache import AttnMeta
 from .config import DeltaConfig
 from .layers import DeltaMapping
@@ -31,6 +31,42 @@ class Sequence:
     arrival: float = 0.0
     prompt: Optional[torch.Tensor] = None
     first_token_time: Optional[float] = None
+
+
+class Hypothesis(NamedTuple):
+    """A finished continuation of a beam search."""
+    tokens: List[int]
+    score: float                        # log-probability / length ** length_penalty
+
+
+class _Beams:
+    """The search for one prompt: its running hypotheses, best first, and what has ended."""
+
+    def __init__(self, number: int, root: Sequence):
+        self.number, self.root, self.first_id = number, root, root.seq_id
+        self.seqs, self.tokens, self.scores = [root], [[]], [0.0]
+        self.common = 0                 # leading cache blocks that all hypotheses hold
+        self.ended: List[Hypothesis] = []
+
+    def end(self, tokens: List[int], score: float, keep: int, penalty: float) -> None:
+        self.ended.append(Hypothesis(tokens, score / len(tokens) ** penalty))
+        self.ended.sort(key=lambda h: -h.score)
+        del self.ended[keep:]
+
+    def decided(self, keep: int, max_new: int, penalty: float) -> bool:
+        """Whether no running hypothesis can still pass the worst of `keep` that have ended: its log-probability only
+        falls, and a longer continuation is divided by more."""
+        if len(self.ended) < keep or not self.scores:
+            return not self.scores
+        length = max_new if penalty > 0 else len(self.tokens[0]) + 1
+        return self.scores[0] / length ** penalty <= self.ended[-1].score
+
+    def shared_blocks(self) -> int:
+        blocks = [s.blocks for s in self.seqs]
+        most = min(map(len, blocks))
+        while self.common < most and len({b[self.common] for b in blocks}) == 1:
+            self.common += 1
+        return self.common
 
 
 class DecodeEngine:
@@ -63,6 +99,7 @@ class DecodeEngine:
         self.positions = None
         self.block_tables = None
         self.attn_splits = 0            # 0: chosen per step from the batch (see decode_step)
+        self.groups = None              # sequences of the batch that share blocks: (sizes, shared lengths), see beam_search
         self.swap_ins = 0
 
     # -- batch composition -----------------------------------------------------------
@@ -161,6 +198,12 @@ class DecodeEngine:
         self.running.remove(seq)
         self._dirty = True
 
+    def compact(self) -> int:
+        """Moves the cache blocks in use to the lowest numbers; returns how many there are."""
+        used = self.cache.compact(self.running)
+        self._dirty = True
+        return used
+
     def _slot_of(self, delta_id: int) -> int:
         return self.manager.delta_index_to_id.index(delta_id) if delta_id > 0 else -1
 
@@ -207,11 +250,10 @@ class DecodeEngine:
         self._dirty = False
 
     # -- one decode step ---------------------------------------------------------------
-    @torch.inference_mode()
-    def decode_step(self) -> torch.Tensor:
-        """Feeds every running sequence its latest token (position = its cached length), appends
-        the new key/value to the cache and samples the next token greedily.  Device work only
-        unless the batch composition changed since the last step."""
+    def _decode_rows(self) -> torch.Tensor:
+        """Feeds every running sequence its latest token; returns the hidden states, rows in the batch's order."""
+        if self.cache.own([(s, 1) for s in self.running]):
+            self._dirty = True
         if self._dirty:
             self._rebuild()
         bs = self.block_size
@@ -223,15 +265,26 @@ class DecodeEngine:
         # one CTA per (sequence, kv head, split): split the keys when the batch alone would leave
         # most SMs without a CTA
         splits = self.attn_splits or max(1, min(8, 296 // max(1, len(self.running) * self.model.kv_heads)))
-        h = self.model(self.tokens, pos, self.cache,
-                       AttnMeta(slot_mapping=slot, block_tables=self.block_tables, seq_lens=lens,
-                                splits=splits, q_starts=self.q_starts, ctx_lens=pos.to(torch.int32),
-                                state_slots=self.state_slots))
-        self.tokens = self.model.greedy_tokens(h)
+        meta = AttnMeta(slot_mapping=slot, block_tables=self.block_tables, seq_lens=lens,
+                        splits=splits, q_starts=self.q_starts, ctx_lens=pos.to(torch.int32),
+                        state_slots=self.state_slots)
+        if self.groups is not None:
+            sizes, shared = self.groups
+            meta.group_starts = self._int32([0] + torch.tensor(sizes).cumsum(0).tolist())
+            meta.shared_lens, meta.max_group, meta.max_shared = self._int32(shared), max(sizes), max(shared)
+        h = self.model(self.tokens, pos, self.cache, meta)
         self.positions = pos + 1
         for s in self.running:
             s.length += 1
             s.generated += 1
+        return h
+
+    @torch.inference_mode()
+    def decode_step(self) -> torch.Tensor:
+        """Feeds every running sequence its latest token (position = its cached length), appends
+        the new key/value to the cache and samples the next token greedily.  Device work only
+        unless the batch composition changed since the last step."""
+        self.tokens = self.model.greedy_tokens(self._decode_rows())
         return self.tokens
 
     # -- given tokens --------------------------------------------------------------------
@@ -273,6 +326,7 @@ class DecodeEngine:
         `max_prefill_tokens` rows."""
         for s, toks in work:
             self.cache.reserve(s, s.length + len(toks))
+        self.cache.own([(s, len(toks)) for s, toks in work])
         order = sorted(range(len(work)), key=lambda i: self._sort_key(work[i][0]))
         limit = self.max_prefill_tokens if self.model.supports_portions else None
         parts: List[List[torch.Tensor]] = [[] for _ in work]
@@ -347,3 +401,120 @@ class DecodeEngine:
                 toks = self.decode_step().tolist()
                 take(toks, self._order, set(self._order))
         return out
+
+    # -- beam search ---------------------------------------------------------------------
+    def _most_blocks(self, prompt: int, max_new: int, beams: int) -> int:
+        """Cache blocks that the hypotheses of a prompt hold at most: full blocks of the prompt together, the rest each by
+        itself (a ring is written all over)."""
+        total = self.cache.blocks_for(prompt + max_new)
+        common = prompt // self.block_size if self.cache.window is None else 0
+        return common + beams * (total - common)
+
+    @torch.inference_mode()
+    def beam_search(self, prompts: List[List[int]], max_new: int, beams: int, delta_ids: Optional[List[int]] = None,
+                    stop_id: Optional[int] = None, length_penalty: float = 1.0) -> List[List[Hypothesis]]:
+        """The best continuations of each prompt by log-probability / length ** length_penalty that a search with `beams`
+        hypotheses finds, best first: of up to `max_new` tokens, or ending in `stop_id`.  Hypotheses share the cache blocks
+        of what they have in common, fork by sharing, and copy a block only before they write to it; recurrent states are
+        copied.  Prompts join as batch slots (`beams` each), cache and deltas allow."""
+        if self.running:
+            raise RuntimeError("sequences are already running")
+        if max_new < 1 or any(not p for p in prompts):
+            raise ValueError("prompts hold at least a token, and at least one token is generated")
+        if not 1 <= beams <= min(self.max_seqs, 64):
+            raise ValueError(f"between 1 and {min(self.max_seqs, 64)} hypotheses a prompt")
+        waiting = [_Beams(i, Sequence(i * beams, delta_ids[i] if delta_ids else 0, len(p), max_new,
+                                      prompt=torch.tensor(p, dtype=torch.int64))) for i, p in enumerate(prompts)]
+        need = {g.number: self._most_blocks(g.root.length, max_new, beams) for g in waiting}
+        keep = beams if stop_id is None else 2 * beams          # as many again may end here
+        out: List[List[Hypothesis]] = [[] for _ in prompts]
+        active: List[_Beams] = []
+        try:
+            while waiting or active:
+                fresh = []
+                for g in list(waiting):
+                    if (len(active) + len(fresh) + 1) * beams > self.max_seqs or \
+                            sum(need[x.number] for x in active + fresh + [g]) > self.cache.num_blocks:
+                        break
+                    if self.admit([g.root]):
+                        fresh.append(g)
+                        waiting.remove(g)
+                if fresh:
+                    for g in fresh:
+                        g.root.length = 0
+                    h = self.extend([(g.root, g.root.prompt.tolist()) for g in fresh])
+                    last = torch.tensor([g.root.length for g in fresh], device=self.device).cumsum(0) - 1
+                    active += fresh
+                    self._select(fresh, h[last], keep, beams, max_new, stop_id, length_penalty, active, out)
+                elif not active:
+                    raise RuntimeError("a waiting request fits neither the cache nor the resident deltas")
+                if active:
+                    self._rebuild_beams(active)
+                    self._select(active, self._decode_rows(), keep, beams, max_new, stop_id, length_penalty, active, out)
+        finally:
+            self.groups = None
+            for s in list(self.running):
+                self.retire(s)
+        return out
+
+    def _rebuild_beams(self, active: List[_Beams]) -> None:
+        """The batch of all hypotheses, each prompt's side by side, and what they share."""
+        self.cache.own([(s, 1) for g in active for s in g.seqs])
+        self._order, tokens = [], {}
+        for g in active:
+            for i, s in enumerate(g.seqs):
+                s.seq_id = g.first_id + i
+                tokens[s.seq_id] = g.tokens[i][-1]
+        self._rebuild(tokens)
+        active.sort(key=lambda g: self._sort_key(g.seqs[0]))
+        self.groups = ([len(g.seqs) for g in active],
+                       [min(g.shared_blocks() * self.block_size, min(s.length for s in g.seqs)) if self.cache.window is None else 0
+                        for g in active])
+
+    def _select(self, groups: List[_Beams], hidden: torch.Tensor, keep: int, beams: int, max_new: int, stop_id: Optional[int],
+                penalty: float, active: List[_Beams], out: List[List[Hypothesis]]) -> None:
+        """Continues the hypotheses of `groups` (their hidden states in this order) by their best next tokens; groups that
+        are through leave `active` with their results."""
+        starts = [0]
+        for g in groups:
+            starts.append(starts[-1] + len(g.seqs))
+        scores = torch.tensor([x for g in groups for x in g.scores], dtype=torch.float32).to(self.device)
+        best = ops.beam_select(self.model.beam_logits(hidden), scores, self._int32(starts), keep)
+        best_scores, rows, tokens = (t.tolist() for t in best)
+        forks = []
+        for i, g in enumerate(list(groups)):
+            nxt = []
+            for rank, (score, row, token) in enumerate(zip(best_scores[i], rows[i], tokens[i])):
+                if score == float("-inf") or len(nxt) == beams:
+                    break
+                parent = row - starts[i]
+                if token != stop_id:
+                    nxt.append((parent, g.tokens[parent] + [token], score))
+                elif rank < beams:
+                    g.end(g.tokens[parent] + [token], score, beams, penalty)
+            if nxt and len(nxt[0][1]) == max_new:
+                for _, toks, score in nxt:
+                    g.end(toks, score, beams, penalty)
+                nxt = []
+            old, g.tokens, g.scores = g.seqs, [t for _, t, _ in nxt], [x for _, _, x in nxt]
+            through = g.decided(beams, max_new, penalty)
+            heirs = set() if through else {p for p, _, _ in nxt}
+            for p, s in enumerate(old):
+                if p not in heirs:
+                    self.retire(s)
+            if through:
+                out[g.number] = g.ended
+                active.remove(g)
+                continue
+            g.seqs, taken = [], set()
+            for p, _, _ in nxt:                                 # the first heir takes the sequence itself
+                if p in taken:
+                    child = Sequence(-1, old[p].delta_id, old[p].length, max_new, generated=old[p].generated)
+                    forks.append((old[p], child))
+                    g.seqs.append(child)
+                else:
+                    taken.add(p)
+                    g.seqs.append(old[p])
+        self.cache.fork(forks)
+        self.running.extend(child for _, child in forks)
+        self._dirty = True

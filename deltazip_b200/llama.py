@@ -150,6 +150,10 @@ class LlamaForCausalLM(nn.Module):
         ops.rotary_and_cache(qkv, positions, self.q_heads, self.kv_heads, cfg.rope_theta, kc, vc,
                              meta.slot_mapping if cache is not None else None)
         scale = 1.0 / math.sqrt(cfg.head_dim)
+        if meta.prompt_lens is None and meta.group_starts is not None and meta.max_shared > 0:
+            return ops.shared_attention_decode(qkv, kc, vc, meta.block_tables, meta.seq_lens, meta.group_starts,
+                                               meta.shared_lens, meta.max_group, meta.max_shared, self.q_heads,
+                                               self.kv_heads, cache.block_size, scale)
         if meta.prompt_lens is None:
             return ops.paged_attention_decode(qkv, kc, vc, meta.block_tables, meta.seq_lens,
                                               self.q_heads, self.kv_heads, cache.block_size, scale,
@@ -199,6 +203,12 @@ class LlamaForCausalLM(nn.Module):
     def logits(self, hidden_last: torch.Tensor) -> torch.Tensor:
         """fp32 logits over this rank's vocabulary rows (sampler math, not the hot path)."""
         return hidden_last.float() @ self.lm_head.float().t()
+
+    def beam_logits(self, hidden: torch.Tensor) -> torch.Tensor:
+        """What a beam search selects from: 32-bit sums of the 16-bit operands' products, over the whole vocabulary."""
+        if self.lm_head.shape[0] != self.cfg.vocab_size:
+            raise ValueError("a beam search needs the whole vocabulary on one rank")
+        return ops.matmul_f32(hidden, self.lm_head)
 
     def greedy_tokens(self, hidden_last: torch.Tensor) -> torch.Tensor:
         """argmax over the whole vocabulary: the output matrix runs on the dense tcgen05 GEMM,
