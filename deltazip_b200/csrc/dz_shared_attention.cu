@@ -4,13 +4,18 @@
 //   out[s, h] = softmax over t of (q[s, h] . k[t] scale) v[t],  t < shared[g] in the group's common pages, the rest in
 //   the sequence's own.
 //
-// Bound: the cache's bytes, shared ones once a group.  The softmax of a row is joined from parts: a part is some of the
-// shared keys for all rows (sequence, query head) of a group that have one key/value head, or some of a sequence's own
-// keys for its query heads, and leaves a maximum, a sum and an unscaled output.  A second launch joins them; nothing is
-// counted or waited for between CTAs.
+// Bound: the cache's bytes, shared ones once a group.  The softmax of a row is joined from parts: a part is a span of
+// the shared keys for up to 64 rows (sequence, query head) of a group that have one key/value head, or a span of a
+// sequence's own keys for its query heads, and leaves a maximum, a sum and an unscaled output.  A second launch joins
+// them; nothing is counted or waited for between CTAs.
 //
-// Rows are those of 16 x 8 x 16 warp MMAs.  A CTA is four warps; with more than 16 rows two or four of them take 16 rows
-// each over the same keys (key tiles in shared memory are theirs together), with fewer they share the keys out.
+// One CTA of eight warps per SM stays for the whole launch.  It first lays out all parts (a scan over groups and
+// sequences in shared memory, the same in every CTA), then its warps take every n-th part: of shared keys in teams of
+// one, two or four warps with 16 rows each over the same key tiles, then of own keys each by itself.  A warp's ring of
+// key tiles runs on from part to part, so that the end of one is not waited for.  Neighbouring parts have
+// neighbouring heads of the same cache rows, and go to different SMs.
+//
+// Rows are those of 16 x 8 x 16 warp MMAs.
 //   scores   S[16 rows, 8 keys] += Q K^T; the order of the 128 products of a score is free, so a lane's 16-byte piece of
 //            a key row serves two MMAs as it lies.
 //   output   O[16 rows, 128] += P V: a 32-bit weight is the sum of three 16-bit parts, all of its bits; the sums of the
@@ -22,12 +27,12 @@ namespace dz {
 namespace {
 
 constexpr int kDim = 128, kRows = 16;                          // rows of a warp
-constexpr int kWarps = 4, kStages = 3, kTile = 16;             // keys per tile
+constexpr int kWarps = 8, kThreads = kWarps * 32, kStages = 3, kTile = 16;     // keys per tile
 constexpr int kRowBytes = kDim * 2, kHalfStage = kTile * kRowBytes, kStageBytes = 2 * kHalfStage;
 constexpr int kRingBytes = kStages * kStageBytes;
-constexpr size_t kSmem = (size_t)kWarps * kRingBytes;
-static_assert(kRingBytes >= kRows * kDim * 4, "a warp's ring also holds its output");
-constexpr int kMaxSplits = 64;
+constexpr int kMaxSeqs = 1536;           // also groups: what the layout of the parts takes of shared memory
+constexpr int kMaxParts = 64;            // of a row
+constexpr int kMinSpan = 64;             // keys of a part: a step of four warps
 
 struct SharedDecode {
   const void* q;
@@ -44,10 +49,11 @@ struct SharedDecode {
   int groups, seqs, heads, kv_heads;
   float scale;
   int max_group, max_shared;
-  int row_groups, row_blocks;            // 16-row blocks of a CTA for shared keys (1, 2, 4), CTAs that a group's rows take
-  int shared_splits, own_splits;
+  int team;                              // warps that take shared keys together (1, 2, 4)
+  int span, parts;                       // keys of a part; parts of a row at most
   float* partial;                        // [sequences, heads, parts, 128]
   float2* ml;                            // [sequences, heads, parts] maximum and sum
+  int* common;                           // [sequences] keys that a sequence reads with its group
 };
 
 // Where 16-byte chunk c of row r lies: rows r, r + 1 in different halves of the banks, any eight consecutive
@@ -73,278 +79,290 @@ __device__ __forceinline__ int shared_keys(const SharedDecode& p, int g) {
 }
 __device__ __forceinline__ int length_of(const SharedDecode& p, int seq) { return min(max(p.lens[seq], 0), p.width * p.block_size); }
 
-// The shared keys that sequence `seq` reads with its group (0: none, it reads all of its keys by itself) and the
-// group's first sequence.  Both launches and both kinds of CTAs go by this alone.
-__device__ __forceinline__ int common_keys(const SharedDecode& p, int seq, int& group) {
-  int lo = 0, hi = p.groups - 1;                               // the last group that starts at or before seq
+// The last of `n` entries that starts at or before x.
+__device__ __forceinline__ int last_before(const int* starts, int n, int x) {
+  int lo = 0, hi = n - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (p.starts[mid] <= seq) lo = mid; else hi = mid - 1;
+    if (starts[mid] <= x) lo = mid; else hi = mid - 1;
   }
-  group = lo;
+  return lo;
+}
+// The shared keys that sequence `seq` reads with its group (0: none, it reads all of its keys by itself).
+__device__ __forceinline__ int common_keys(const SharedDecode& p, const int* starts, int seq) {
   if (p.groups == 0) return 0;
-  const int first = p.starts[lo];
-  if (first < 0 || seq < first || seq >= p.starts[lo + 1] || seq - first >= p.max_group) return 0;
-  const int n = shared_keys(p, lo);
+  const int g = last_before(starts, p.groups, seq), first = starts[g];
+  if (first < 0 || seq < first || seq >= starts[g + 1] || seq - first >= p.max_group) return 0;
+  const int n = shared_keys(p, g);
   return length_of(p, seq) >= n ? n : 0;
 }
 
-// Keys of a part, and parts that `keys` keys take: a step of a CTA is four tiles, no part has fewer.
-__device__ __forceinline__ int part_keys(int keys, int splits) {
-  return max(((keys + splits - 1) / splits + kTile - 1) / kTile * kTile, kWarps * kTile);
-}
-__device__ __forceinline__ int part_count(int keys, int splits) {
-  const int per = part_keys(keys, splits);
-  return (keys + per - 1) / per;
+// Running sums of count(i), i < n, in front of each i and at sums[n].  Every thread of the block calls it.
+template <typename F>
+__device__ __forceinline__ void lay_out(int n, int* sums, int* warp_sums, F count) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int before = 0;
+  for (int i0 = 0; i0 < n; i0 += kThreads) {
+    const int i = i0 + threadIdx.x, c = i < n ? count(i) : 0;
+    int upto = c;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += up;
+    }
+    if (lane == 31) warp_sums[warp] = upto;
+    __syncthreads();
+    int ahead = before, all = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      ahead += w < warp ? warp_sums[w] : 0;
+      all += warp_sums[w];
+    }
+    if (i < n) sums[i] = ahead + upto - c;
+    before += all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) sums[n] = before;
 }
 
+// A span of keys for some rows.
+struct Part {
+  int kvh, t0, t1, tiles;
+  int source;                            // the sequence in whose table the keys are
+  int seq0, row0, rows;                  // rows (seq0 + r / ratio, kvh * ratio + r % ratio), row0 <= r < rows
+  int index;                             // among the parts of a row
+};
+
 template <typename T>
-__global__ void __launch_bounds__(kWarps * 32, 2) shared_decode_kernel(SharedDecode p) {
+__global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(SharedDecode p) {
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows];
+  __shared__ int s_warp[kWarps];
+  int* s_starts = reinterpret_cast<int*>(smem + kWarps * kRingBytes);    // [groups + 1]
+  int* s_source = s_starts + p.groups + 1;                    // [groups] first sequence that has all the shared keys
+  int* s_shared = s_source + p.groups;                        // [groups + 1] parts of shared keys, over heads
+  int* s_common = s_shared + p.groups + 1;                    // [sequences]
+  int* s_own = s_common + p.seqs;                             // [sequences + 1] parts of own keys
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gq = lane >> 2, t = lane & 3;
   const int ratio = p.heads / p.kv_heads;
   pdl_wait();
   pdl_launch();
-  // which part: CTAs of shared keys first, neighbours with neighbouring pieces of the same cache rows
-  int at = blockIdx.x;
-  const int shared_ctas = p.groups * p.shared_splits * p.row_blocks * p.kv_heads;
-  const bool own = at >= shared_ctas;
-  if (own) at -= shared_ctas;
-  const int kvh = at % p.kv_heads;
-  at /= p.kv_heads;
-  int seq0, source, rows, row0 = 0, lo, len, splits, split, rg, group = -1;
-  if (own) {
-    splits = p.own_splits;
-    split = at % splits;
-    seq0 = source = at / splits;
-    rg = 1;
-    rows = ratio;
-    int g;
-    lo = common_keys(p, seq0, g);
-    len = length_of(p, seq0);
-  } else {
-    rg = p.row_groups;
-    row0 = at % p.row_blocks * rg * kRows;
-    at /= p.row_blocks;
-    splits = p.shared_splits;
-    split = at % splits;
-    group = at / splits;
-    seq0 = source = p.starts[group];
-    const int last = min(p.starts[group + 1], p.seqs);
-    if (seq0 < 0 || seq0 >= last) return;
-    const int seqs = min(last - seq0, p.max_group);
-    rows = seqs * ratio;
-    lo = 0;
-    len = shared_keys(p, group);
-    if (row0 >= rows) return;
-    while (source < seq0 + seqs && length_of(p, source) < len) ++source;      // whose pages hold all the shared keys
-    if (source == seq0 + seqs) return;
-  }
-  const int per = part_keys(len - lo, splits);
-  const int t0 = lo + split * per, t1 = min(len, t0 + per);
-  // (an empty row: its first part writes zeros)
-  const bool empty = own && len == 0 && split == 0;
-  if (t0 >= t1 && !empty) return;
-  const int* table = p.tables + (size_t)source * p.width;
-  const T* kc = (const T*)p.k_cache;
-  const T* vc = (const T*)p.v_cache;
-  uint8_t* ring = smem + warp * kRingBytes;
-  const int kg = warp / rg, first_warp = kg * rg;              // warps that share key tiles
-
-  // cache row of key t0 + 16 * tile + (lane & 15); keys past the end repeat the last one
-  auto row_of = [&](int tile) {
-    const int k = min(t0 + tile * kTile + (lane & 15), t1 - 1), b = k / p.block_size;
-    const int64_t r = (int64_t)table[b] * p.block_size + (k - b * p.block_size);
-    return min(max(r, (int64_t)0), p.cache_rows - 1);
-  };
-  auto issue = [&](int stage, int tile, int64_t row) {
-    const int c = lane & 15, keys = t1 - t0 - tile * kTile;    // values past the end are zero, as their weights are
-#pragma unroll
-    for (int j = 0; j < kTile / 2; ++j) {
-      const int r = 2 * j + (lane >> 4);
-      const int64_t from = (__shfl_sync(0xffffffffu, row, r) * p.kv_heads + kvh) * kDim + c * 8;
-      uint8_t* dst = ring + stage * kStageBytes + chunk_at(r, c);
-      cp_async16(dst, kc + from, true);
-      cp_async16(dst + kHalfStage, vc + from, r < keys);
-    }
-  };
-  const int tiles = empty ? 0 : (t1 - t0 + kTile - 1) / kTile;
-  int64_t next = 0;                                            // row of the tile that is requested next
-  if (warp < tiles) next = row_of(warp);
-#pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) {
-    const int tile = warp + s * kWarps;
-    if (tile < tiles) {
-      issue(s, tile, next);
-      if (tile + kWarps < tiles) next = row_of(tile + kWarps);
-    }
-    cp_async_commit();
-  }
-
-  // rows gq and gq + 8 of the warp's 16: components 32 c + 8 t ... + 7; absent rows are zero
-  const int mine = row0 + (warp - first_warp) * kRows;
-  uint4 q[2][4];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = mine + gq + 8 * i;
-    const T* from = (const T*)p.q + (size_t)(seq0 + r / ratio) * p.q_stride + (size_t)(kvh * ratio + r % ratio) * kDim;
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-      q[i][c] = r < rows ? *reinterpret_cast<const uint4*>(from + c * 32 + t * 8) : make_uint4(0, 0, 0, 0);
-  }
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  float o[16][4], o2[16][4];                                   // [8 components][row gq: 2, row gq + 8: 2]: first parts, others
-#pragma unroll
-  for (int j = 0; j < 16; ++j)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[j][e] = o2[j][e] = 0.f;
-
-  int stage = 0;
-  for (int step = 0; step * kWarps + first_warp < tiles; ++step) {
-    cp_async_wait<kStages - 2>();
-    if (rg == 1) __syncwarp();
-    else asm volatile("bar.sync %0, %1;" ::"r"(kg + 1), "r"(rg * 32) : "memory");
-    {
-      const int ahead = (step + kStages - 1) * kWarps + warp;
-      if (ahead < tiles) {
-        issue(stage == 0 ? kStages - 1 : stage - 1, ahead, next);
-        if (ahead + kWarps < tiles) next = row_of(ahead + kWarps);
-      }
-      cp_async_commit();
-    }
-    for (int w = 0; w < rg; ++w) {
-      const int tile = step * kWarps + first_warp + w;
-      if (tile >= tiles) break;
-      const uint8_t* ks = smem + (first_warp + w) * kRingBytes + stage * kStageBytes;
-      const int k0 = t0 + tile * kTile;
-      float x[2][2][2];                                        // [keys k0 + 8 i][row gq + 8 h][key 2 t + e]
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const uint4 k = *reinterpret_cast<const uint4*>(ks + chunk_at(i * 8 + gq, 4 * c + t));
-          const uint32_t a0[4] = {q[0][c].x, q[1][c].x, q[0][c].y, q[1][c].y};
-          const uint32_t a1[4] = {q[0][c].z, q[1][c].z, q[0][c].w, q[1][c].w};
-          mma16816<T>(s[0], a0, k.x, k.y);
-          mma16816<T>(s[1], a1, k.z, k.w);
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) x[i][h][e] = (s[0][2 * h + e] + s[1][2 * h + e]) * p.scale;
-      }
-      if (k0 + kTile > t1) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if (k0 + i * 8 + 2 * t + e >= t1) x[i][0][e] = x[i][1][e] = -INFINITY;
-      }
-      float ms[2], c[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float mx = fmaxf(fmaxf(x[0][h][0], x[0][h][1]), fmaxf(x[1][h][0], x[1][h][1]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float mn = fmaxf(m[h], mx);
-        ms[h] = mn == -INFINITY ? 0.f : mn;
-        c[h] = mn == m[h] ? 1.f : __expf(m[h] - ms[h]);
-        m[h] = mn;
-      }
-      if (__any_sync(0xffffffffu, c[0] != 1.f || c[1] != 1.f)) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) l[h] *= c[h];
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            o[j][e] *= c[e >> 1];
-            o2[j][e] *= c[e >> 1];
-          }
-      }
-      uint32_t hi[4], mid[4], low[4];
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float w0 = __expf(x[i][h][0] - ms[h]), w1 = __expf(x[i][h][1] - ms[h]);
-          l[h] += w0 + w1;
-          split_weights<T>(w0, w1, hi[2 * i + h], mid[2 * i + h], low[2 * i + h]);
-        }
-      const uint8_t* vs = ks + kHalfStage;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        uint32_t b[4];
-        ldsm4_t(b, vs + chunk_at(lane & 15, 2 * j + (lane >> 4)));
-        mma16816<T>(o[2 * j], hi, b[0], b[1]);
-        mma16816<T>(o[2 * j + 1], hi, b[2], b[3]);
-        mma16816<T>(o2[2 * j], mid, b[0], b[1]);
-        mma16816<T>(o2[2 * j + 1], mid, b[2], b[3]);
-        mma16816<T>(o2[2 * j], low, b[0], b[1]);
-        mma16816<T>(o2[2 * j + 1], low, b[2], b[3]);
-      }
-    }
-    stage = stage == kStages - 1 ? 0 : stage + 1;
-  }
-  cp_async_wait<0>();
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-  }
-  __syncthreads();                                             // the warps' rings become their outputs [16, 128]
-  float* out = reinterpret_cast<float*>(ring);
-  // where the values held an infinity, the first parts' products are the result and the others' may be anything
-  auto whole = [](float a, float b) { return (isfinite(a) ? a + b : a) * (1.f / kScale<T>); };
-#pragma unroll
-  for (int j = 0; j < 16; ++j)
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      *reinterpret_cast<float2*>(out + (gq + 8 * h) * kDim + j * 8 + 2 * t) =
-          make_float2(whole(o[j][2 * h], o2[j][2 * h]), whole(o[j][2 * h + 1], o2[j][2 * h + 1]));
-  if (t == 0) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      s_m[warp][gq + 8 * h] = m[h];
-      s_l[warp][gq + 8 * h] = l[h];
-    }
-  }
+  for (int i = threadIdx.x; i <= p.groups; i += kThreads) s_starts[i] = p.groups ? p.starts[i] : 0;
+  __syncthreads();
+  const int block_rows = p.team * kRows;
+  lay_out(p.groups, s_shared, s_warp, [&](int g) {
+    const int first = s_starts[g], keys = shared_keys(p, g);
+    s_source[g] = first;
+    if (first < 0 || first >= p.seqs || keys == 0) return 0;
+    const int n = min(min(max(s_starts[g + 1], first), p.seqs) - first, p.max_group);
+    int source = first;
+    while (source < first + n && length_of(p, source) < keys) ++source;
+    s_source[g] = source;
+    return source < first + n ? (keys + p.span - 1) / p.span * ((n * ratio + block_rows - 1) / block_rows) : 0;
+  });
+  lay_out(p.seqs, s_own, s_warp, [&](int seq) {
+    const int common = common_keys(p, s_starts, seq);
+    s_common[seq] = common;
+    if (blockIdx.x == 0) p.common[seq] = common;
+    return (length_of(p, seq) - common + p.span - 1) / p.span;
+  });
   __syncthreads();
 
-  // four components of a row per thread and round
-  const int parts = p.shared_splits + p.own_splits;
-  const int part = own ? p.shared_splits + split : split;
-  const bool alone = own && lo == 0 && (empty || part_count(len, splits) == 1);      // nothing to join
-  const int live = min(rows - row0, rg * kRows);
-  for (int i = threadIdx.x * 4; i < live * kDim; i += kWarps * 32 * 4) {
-    const int r = i / kDim, d = i % kDim, w0 = r / kRows, rr = r % kRows;
-    const int seq = seq0 + (row0 + r) / ratio, head = kvh * ratio + (row0 + r) % ratio;
-    if (!own) {
-      int g;
-      if (common_keys(p, seq, g) == 0 || g != group) continue; // it reads all of its keys by itself
+  const T* kc = (const T*)p.k_cache;
+  const T* vc = (const T*)p.v_cache;
+  for (int phase = 0; phase < 2; ++phase) {
+    const bool own = phase == 1;
+    const int team = own ? 1 : p.team, member = warp % team, first_warp = warp - member;
+    const int teams = gridDim.x * (kWarps / team);
+    const int units = (int)min((int64_t)(own ? s_own[p.seqs] : s_shared[p.groups]) * p.kv_heads, (int64_t)1 << 30);
+    // (the second phase in the other direction: who had a part more then has one less)
+    int unit = warp / team * gridDim.x + blockIdx.x;
+    if (own) unit = teams - 1 - unit;
+
+    auto part_of = [&](int u) {
+      Part x;
+      x.kvh = u % p.kv_heads;
+      const int v = u / p.kv_heads;
+      if (own) {
+        const int seq = last_before(s_own, p.seqs, v), chunk = v - s_own[seq], common = s_common[seq];
+        x.source = x.seq0 = seq;
+        x.row0 = 0;
+        x.rows = ratio;
+        x.t0 = common + chunk * p.span;
+        x.t1 = min(length_of(p, seq), x.t0 + p.span);
+        x.index = (common + p.span - 1) / p.span + chunk;
+      } else {
+        const int g = last_before(s_shared, p.groups, v), i = v - s_shared[g];
+        x.seq0 = s_starts[g];
+        x.source = s_source[g];
+        x.rows = min(min(s_starts[g + 1], p.seqs) - x.seq0, p.max_group) * ratio;
+        const int blocks = (x.rows + block_rows - 1) / block_rows;
+        x.row0 = i % blocks * block_rows;
+        x.index = i / blocks;
+        x.t0 = x.index * p.span;
+        x.t1 = min(shared_keys(p, g), x.t0 + p.span);
+      }
+      x.tiles = (x.t1 - x.t0 + kTile - 1) / kTile;
+      return x;
+    };
+
+    // The ring: what is requested runs kStages - 1 steps (a tile of every warp of the team) ahead of what is used.
+    uint8_t* ring = smem + warp * kRingBytes;
+    int ahead_unit = unit, ahead_step = 0, stage = 0;
+    Part ahead;
+    int64_t row = 0;                                           // cache row of key 16 * tile + (lane & 15) of the next request
+    auto find_row = [&]() {
+      const int tile = ahead_step * team + member;
+      if (ahead_unit >= units || tile >= ahead.tiles) return;
+      const int k = min(ahead.t0 + tile * kTile + (lane & 15), ahead.t1 - 1), b = k / p.block_size;   // keys past the end repeat the last
+      const int64_t r = (int64_t)p.tables[(size_t)ahead.source * p.width + b] * p.block_size + (k - b * p.block_size);
+      row = min(max(r, (int64_t)0), p.cache_rows - 1);
+    };
+    auto request = [&](int to) {                               // and go on to the next one
+      const int tile = ahead_step * team + member;
+      if (ahead_unit < units) {
+        if (tile < ahead.tiles) {
+          const int c = lane & 15, keys = ahead.t1 - ahead.t0 - tile * kTile;  // values past the end are zero, as their weights are
+#pragma unroll
+          for (int j = 0; j < kTile / 2; ++j) {
+            const int r = 2 * j + (lane >> 4);
+            const int64_t from = (__shfl_sync(0xffffffffu, row, r) * p.kv_heads + ahead.kvh) * kDim + c * 8;
+            uint8_t* dst = ring + to * kStageBytes + chunk_at(r, c);
+            cp_async16(dst, kc + from, true);
+            cp_async16(dst + kHalfStage, vc + from, r < keys);
+          }
+        }
+        if (++ahead_step * team >= ahead.tiles) {
+          ahead_step = 0;
+          ahead_unit += teams;
+          if (ahead_unit < units) ahead = part_of(ahead_unit);
+        }
+        find_row();
+      }
+      cp_async_commit();
+    };
+    if (unit < units) ahead = part_of(unit);
+    find_row();
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) request(s);
+
+    for (; unit < units; unit += teams) {
+      const Part part = part_of(unit);
+      // rows gq and gq + 8 of the warp's 16: components 32 c + 8 t ... + 7; absent rows are zero
+      const int mine = part.row0 + member * kRows;
+      uint4 q[2][4];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = mine + gq + 8 * i;
+        const T* from = (const T*)p.q + (size_t)(part.seq0 + r / ratio) * p.q_stride + (size_t)(part.kvh * ratio + r % ratio) * kDim;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          q[i][c] = r < part.rows ? *reinterpret_cast<const uint4*>(from + c * 32 + t * 8) : make_uint4(0, 0, 0, 0);
+      }
+      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+      float o[16][4], o2[16][4];                               // [8 components][row gq: 2, row gq + 8: 2]: first parts, others
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[j][e] = o2[j][e] = 0.f;
+
+      for (int step = 0; step * team < part.tiles; ++step) {
+        cp_async_wait<kStages - 2>();
+        if (team == 1) __syncwarp();
+        else asm volatile("bar.sync %0, %1;" ::"r"(first_warp / team + 1), "r"(team * 32) : "memory");
+        request(stage == 0 ? kStages - 1 : stage - 1);
+        for (int w = 0; w < team; ++w) {
+          const int tile = step * team + w;
+          if (tile >= part.tiles) break;
+          const uint8_t* ks = smem + (first_warp + w) * kRingBytes + stage * kStageBytes;
+          const int k0 = part.t0 + tile * kTile;
+          float x[2][2][2];                                    // [keys k0 + 8 i][row gq + 8 h][key 2 t + e]
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const uint4 k = *reinterpret_cast<const uint4*>(ks + chunk_at(i * 8 + gq, 4 * c + t));
+              const uint32_t a0[4] = {q[0][c].x, q[1][c].x, q[0][c].y, q[1][c].y};
+              const uint32_t a1[4] = {q[0][c].z, q[1][c].z, q[0][c].w, q[1][c].w};
+              mma16816<T>(s[0], a0, k.x, k.y);
+              mma16816<T>(s[1], a1, k.z, k.w);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) x[i][h][e] = (s[0][2 * h + e] + s[1][2 * h + e]) * p.scale;
+          }
+          if (k0 + kTile > part.t1) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                if (k0 + i * 8 + 2 * t + e >= part.t1) x[i][0][e] = x[i][1][e] = -INFINITY;
+          }
+          float ms[2], c[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float mx = fmaxf(fmaxf(x[0][h][0], x[0][h][1]), fmaxf(x[1][h][0], x[1][h][1]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            const float mn = fmaxf(m[h], mx);
+            ms[h] = mn == -INFINITY ? 0.f : mn;
+            c[h] = mn == m[h] ? 1.f : __expf(m[h] - ms[h]);
+            m[h] = mn;
+          }
+          if (__any_sync(0xffffffffu, c[0] != 1.f || c[1] != 1.f)) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) l[h] *= c[h];
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                o[j][e] *= c[e >> 1];
+                o2[j][e] *= c[e >> 1];
+              }
+          }
+          uint32_t hi[4], mid[4], low[4];
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float w0 = __expf(x[i][h][0] - ms[h]), w1 = __expf(x[i][h][1] - ms[h]);
+              l[h] += w0 + w1;
+              split_weights<T>(w0, w1, hi[2 * i + h], mid[2 * i + h], low[2 * i + h]);
+            }
+          const uint8_t* vs = ks + kHalfStage;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            uint32_t b[4];
+            ldsm4_t(b, vs + chunk_at(lane & 15, 2 * j + (lane >> 4)));
+            mma16816<T>(o[2 * j], hi, b[0], b[1]);
+            mma16816<T>(o[2 * j + 1], hi, b[2], b[3]);
+            mma16816<T>(o2[2 * j], mid, b[0], b[1]);
+            mma16816<T>(o2[2 * j + 1], mid, b[2], b[3]);
+            mma16816<T>(o2[2 * j], low, b[0], b[1]);
+            mma16816<T>(o2[2 * j + 1], low, b[2], b[3]);
+          }
+        }
+        stage = stage == kStages - 1 ? 0 : stage + 1;
+      }
+      // where the values held an infinity, the first parts' products are the result and the others' may be anything
+      auto whole = [](float a, float b) { return (isfinite(a) ? a + b : a) * (1.f / kScale<T>); };
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+        const int r = mine + gq + 8 * h, seq = part.seq0 + r / ratio;
+        if (r < part.rows && (own || s_common[seq] > 0)) {     // (otherwise it reads all of its keys by itself)
+          const size_t to = ((size_t)seq * p.heads + part.kvh * ratio + r % ratio) * p.parts + part.index;
+          float* out = p.partial + to * kDim + 2 * t;
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            *reinterpret_cast<float2*>(out + j * 8) = make_float2(whole(o[j][2 * h], o2[j][2 * h]), whole(o[j][2 * h + 1], o2[j][2 * h + 1]));
+          if (t == 0) p.ml[to] = make_float2(m[h], l[h]);
+        }
+      }
     }
-    float mm = -INFINITY, sum = 0.f, a[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int w = w0; w < kWarps; w += rg) mm = fmaxf(mm, s_m[w][rr]);
-    for (int w = w0; w < kWarps; w += rg) {
-      const float c = s_m[w][rr] == -INFINITY ? 0.f : __expf(s_m[w][rr] - mm);
-      const float4 v = *reinterpret_cast<const float4*>(smem + w * kRingBytes + (size_t)(rr * kDim + d) * 4);
-      sum += s_l[w][rr] * c;
-      a[0] += v.x * c;
-      a[1] += v.y * c;
-      a[2] += v.z * c;
-      a[3] += v.w * c;
-    }
-    const size_t to = (size_t)seq * p.heads + head;
-    if (alone) {
-      uint2 v = make_uint2(Cvt<T>::down(a[0] / sum, a[1] / sum), Cvt<T>::down(a[2] / sum, a[3] / sum));
-      if (empty) v = make_uint2(0, 0);
-      *reinterpret_cast<uint2*>((T*)p.out + to * kDim + d) = v;
-    } else {
-      *reinterpret_cast<float4*>(p.partial + (to * parts + part) * kDim + d) = make_float4(a[0], a[1], a[2], a[3]);
-      if (d == 0) p.ml[to * parts + part] = make_float2(mm, sum);
-    }
+    cp_async_wait<0>();
+    if (phase == 0) __syncthreads();                           // the rings change hands
   }
 }
 
@@ -355,20 +373,16 @@ __global__ void __launch_bounds__(256) shared_join_kernel(SharedDecode p) {
   pdl_launch();
   const int row = blockIdx.x * 8 + (threadIdx.x >> 5), d = (threadIdx.x & 31) * 4;
   if (row >= p.seqs * p.heads) return;
-  int g;
-  const int seq = row / p.heads, common = common_keys(p, seq, g), fresh = length_of(p, seq) - common;
-  const int before = common > 0 ? part_count(common, p.shared_splits) : 0, after = fresh > 0 ? part_count(fresh, p.own_splits) : 0;
-  if (before == 0 && after <= 1) return;                       // written already
-  const int parts = p.shared_splits + p.own_splits;
-  const float2* ml = p.ml + (size_t)row * parts;
-  const float* from = p.partial + (size_t)row * parts * kDim + d;
-  auto place = [&](int i) { return i < before ? i : p.shared_splits + i - before; };
+  const int seq = row / p.heads, common = p.common[seq], fresh = length_of(p, seq) - common;
+  const int parts = (common + p.span - 1) / p.span + (fresh + p.span - 1) / p.span;
+  const float2* ml = p.ml + (size_t)row * p.parts;
+  const float* from = p.partial + (size_t)row * p.parts * kDim + d;
   float mm = -INFINITY, sum = 0.f, a[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < before + after; ++i) mm = fmaxf(mm, ml[place(i)].x);
+  for (int i = 0; i < parts; ++i) mm = fmaxf(mm, ml[i].x);
 #pragma unroll 4
-  for (int i = 0; i < before + after; ++i) {
-    const float2 w = ml[place(i)];
-    const float4 v = *reinterpret_cast<const float4*>(from + (size_t)place(i) * kDim);
+  for (int i = 0; i < parts; ++i) {
+    const float2 w = ml[i];
+    const float4 v = *reinterpret_cast<const float4*>(from + (size_t)i * kDim);
     const float c = w.x == -INFINITY ? 0.f : __expf(w.x - mm);
     sum += w.y * c;
     a[0] += v.x * c;
@@ -376,30 +390,37 @@ __global__ void __launch_bounds__(256) shared_join_kernel(SharedDecode p) {
     a[2] += v.z * c;
     a[3] += v.w * c;
   }
-  *reinterpret_cast<uint2*>((T*)p.out + (size_t)row * kDim + d) =
-      make_uint2(Cvt<T>::down(a[0] / sum, a[1] / sum), Cvt<T>::down(a[2] / sum, a[3] / sum));
+  uint2 v = make_uint2(Cvt<T>::down(a[0] / sum, a[1] / sum), Cvt<T>::down(a[2] / sum, a[3] / sum));
+  if (parts == 0) v = make_uint2(0, 0);
+  *reinterpret_cast<uint2*>((T*)p.out + (size_t)row * kDim + d) = v;
 }
 
 struct Plan {
-  int row_groups, row_blocks, shared_splits, own_splits;
+  int team, span, parts;
 };
-// Parts of `most` keys over `columns` CTAs: about four rounds of two CTAs on each SM, of 256 keys or more.
-int parts_for(int64_t columns, int64_t most) {
-  const int64_t want = (4 * 296 + columns - 1) / (columns > 0 ? columns : 1), can = most / 256;
-  const int64_t n = want < can ? want : can;
-  return (int)(n < 1 ? 1 : n > kMaxSplits ? kMaxSplits : n);
-}
 Plan plan(int num_seqs, int num_groups, int max_group, int max_shared, int max_keys, int heads, int kv_heads) {
-  const int ratio = heads / kv_heads, shared = max_shared < max_keys ? max_shared : max_keys;
+  const int ratio = heads / kv_heads;
+  const int64_t shared = max_shared < max_keys ? max_shared : max_keys;
   Plan r;
   const int64_t rows = (int64_t)(max_group < num_seqs ? max_group : num_seqs) * ratio;
-  r.row_groups = rows <= kRows ? 1 : rows <= 2 * kRows ? 2 : 4;
-  r.row_blocks = (int)((rows + r.row_groups * kRows - 1) / (r.row_groups * kRows));
-  r.shared_splits = num_groups > 0 && shared > 0 ? parts_for((int64_t)num_groups * r.row_blocks * kv_heads, shared) : 0;
-  r.own_splits = parts_for((int64_t)num_seqs * kv_heads, max_keys - shared);
+  r.team = rows <= kRows ? 1 : rows <= 2 * kRows ? 2 : 4;
+  // about eight parts for every team, were all lengths two thirds of the longest; no more than a row's table takes
+  const int64_t keys = (num_groups * shared * ((rows + r.team * kRows - 1) / (r.team * kRows)) * r.team + num_seqs * (max_keys - shared)) * kv_heads * 2 / 3;
+  int64_t span = keys / (148 * kWarps * 8);
+  const int64_t least = (max_keys + kMaxParts - 3) / (kMaxParts - 2);
+  if (span < least) span = least;
+  if (span < kMinSpan) span = kMinSpan;
+  r.span = (int)((span + kMinSpan - 1) / kMinSpan * kMinSpan);
+  r.parts = max_keys / r.span + 2;
   return r;
 }
-size_t partial_floats(int num_seqs, int heads, const Plan& r) { return (size_t)num_seqs * heads * (r.shared_splits + r.own_splits) * kDim; }
+struct Scratch {
+  size_t ml, common, total;              // behind the parts' outputs
+};
+Scratch scratch(int num_seqs, int heads, const Plan& r) {
+  const size_t n = (size_t)num_seqs * heads * r.parts;
+  return {n * kDim * 4, n * (kDim * 4 + 8), n * (kDim * 4 + 8) + (size_t)num_seqs * 4};
+}
 
 }  // namespace
 }  // namespace dz
@@ -408,13 +429,14 @@ using namespace dz;
 
 extern "C" {
 
+int dz_shared_attention_max_seqs(void) { return kMaxSeqs; }
+
 size_t dz_shared_attention_workspace_bytes(int num_seqs, int num_groups, int max_group, int max_shared, int max_keys, int q_heads,
                                            int kv_heads) {
   if (num_seqs <= 0 || num_groups < 0 || max_group < 0 || max_shared < 0 || max_keys <= 0 || q_heads <= 0 || kv_heads <= 0 ||
       q_heads % kv_heads)
     return 0;
-  const Plan r = plan(num_seqs, num_groups, max_group, max_shared, max_keys, q_heads, kv_heads);
-  return partial_floats(num_seqs, q_heads, r) * 4 + (size_t)num_seqs * q_heads * (r.shared_splits + r.own_splits) * 8;
+  return scratch(num_seqs, q_heads, plan(num_seqs, num_groups, max_group, max_shared, max_keys, q_heads, kv_heads)).total;
 }
 
 int dz_shared_attention_decode(const dz_shared_attention_args* a, void* stream) {
@@ -432,26 +454,26 @@ int dz_shared_attention_decode(const dz_shared_attention_args* a, void* stream) 
   if ((a->q_row_stride & 7) || !aligned16(a->qkv) || !aligned16(a->out) || !aligned16(a->k_cache) || !aligned16(a->v_cache))
     return DZ_ERR_ALIGNMENT;
   const int64_t keys = (int64_t)a->table_width * a->block_size;
-  if (keys > (1 << 30) || (int64_t)a->num_seqs * a->q_heads > (1 << 26)) return DZ_ERR_TOO_LARGE;
+  if (a->num_seqs > kMaxSeqs || a->num_groups > kMaxSeqs || keys > (1 << 30) || a->kv_heads > 4096) return DZ_ERR_TOO_LARGE;
   const Plan r = plan(a->num_seqs, a->num_groups, a->max_group, a->max_shared, (int)keys, a->q_heads, a->kv_heads);
-  const int64_t ctas = (int64_t)a->num_groups * r.shared_splits * r.row_blocks * a->kv_heads +
-                       (int64_t)a->num_seqs * r.own_splits * a->kv_heads;
-  if (ctas > 0x7fffffff) return DZ_ERR_TOO_LARGE;
+  // parts are counted in 32 bits
+  if ((int64_t)a->num_seqs * 2 * r.parts * a->kv_heads > (1 << 30)) return DZ_ERR_TOO_LARGE;
   if (!a->workspace || a->workspace_bytes < dz_shared_attention_workspace_bytes(a->num_seqs, a->num_groups, a->max_group, a->max_shared,
                                                                                (int)keys, a->q_heads, a->kv_heads))
     return DZ_ERR_WORKSPACE;
   if (!aligned16(a->workspace)) return DZ_ERR_ALIGNMENT;
-  float* partial = reinterpret_cast<float*>(a->workspace);
+  uint8_t* ws = reinterpret_cast<uint8_t*>(a->workspace);
+  const Scratch at = scratch(a->num_seqs, a->q_heads, r);
   const SharedDecode p = {a->qkv, a->q_row_stride, a->out, a->k_cache, a->v_cache, a->cache_rows, a->block_tables, a->table_width,
                           a->block_size, a->seq_lens, a->group_starts, a->shared_lens, a->num_groups, a->num_seqs, a->q_heads,
-                          a->kv_heads, a->scale, a->max_group, a->max_shared, r.row_groups, r.row_blocks, r.shared_splits,
-                          r.own_splits, partial, reinterpret_cast<float2*>(partial + partial_floats(a->num_seqs, a->q_heads, r))};
+                          a->kv_heads, a->scale, a->max_group, a->max_shared, r.team, r.span, r.parts,
+                          reinterpret_cast<float*>(ws), reinterpret_cast<float2*>(ws + at.ml), reinterpret_cast<int*>(ws + at.common)};
   cudaStream_t st = (cudaStream_t)stream;
   const int rows = a->num_seqs * a->q_heads;
-  DZ_DISPATCH16(a->dtype, DZ_CUDA_OK(allow_smem(shared_decode_kernel<T>, kSmem));
-                DZ_CUDA_OK(launch_ex(shared_decode_kernel<T>, dim3((unsigned)ctas), dim3(kWarps * 32), kSmem, 1, st, p));
-                if (r.shared_splits + r.own_splits > 1)
-                    DZ_CUDA_OK(launch_pdl(shared_join_kernel<T>, dim3((rows + 7) / 8), dim3(256), st, p)));
+  const size_t smem = (size_t)kWarps * kRingBytes + (size_t)(3 * a->num_groups + 2 * a->num_seqs + 3) * 4;
+  DZ_DISPATCH16(a->dtype, DZ_CUDA_OK(allow_smem(shared_decode_kernel<T>, smem));
+                DZ_CUDA_OK(launch_ex(shared_decode_kernel<T>, dim3(148), dim3(kThreads), smem, 1, st, p));
+                DZ_CUDA_OK(launch_pdl(shared_join_kernel<T>, dim3((rows + 7) / 8), dim3(256), st, p)));
   return DZ_OK;
 }
 

@@ -150,7 +150,8 @@ class LlamaForCausalLM(nn.Module):
         ops.rotary_and_cache(qkv, positions, self.q_heads, self.kv_heads, cfg.rope_theta, kc, vc,
                              meta.slot_mapping if cache is not None else None)
         scale = 1.0 / math.sqrt(cfg.head_dim)
-        if meta.prompt_lens is None and meta.group_starts is not None and meta.max_shared > 0:
+        if meta.prompt_lens is None and meta.group_starts is not None and meta.max_shared > 0 and \
+                qkv.shape[0] <= ops.shared_attention_max_seqs():
             return ops.shared_attention_decode(qkv, kc, vc, meta.block_tables, meta.seq_lens, meta.group_starts,
                                                meta.shared_lens, meta.max_group, meta.max_shared, self.q_heads,
                                                self.kv_heads, cache.block_size, scale)

@@ -1089,6 +1089,11 @@ def copy_pages_max_pairs() -> int:
     return lib().dz_copy_pages_max_pairs()
 
 
+def shared_attention_max_seqs() -> int:
+    """The most sequences, and groups of them, that a shared_attention_decode takes."""
+    return lib().dz_shared_attention_max_seqs()
+
+
 def shared_attention_decode(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
                             seq_lens: torch.Tensor, group_starts: torch.Tensor, shared_lens: torch.Tensor, max_group: int,
                             max_shared: int, q_heads: int, kv_heads: int, block_size: int, scale: float,

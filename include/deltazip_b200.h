@@ -572,7 +572,7 @@ int dz_moe_gemm(const void* x, const void* weights, const int32_t* offsets, cons
  *                 tables begin alike), which are read once for the first max_group of them.  A sequence shorter than
  *                 that, or outside the groups, is read by itself; shared lengths above max_shared are read as
  *                 max_shared.  1 to 16 query heads per kv head.  A page number outside the cache is read as the
- *                 nearest row of it.  The workspace (dz_shared_attention_workspace_bytes, max_keys = table_width *
+ *                 nearest row of it.  At most dz_shared_attention_max_seqs() sequences and groups.  The workspace (dz_shared_attention_workspace_bytes, max_keys = table_width *
  *                 block_size) needs no preparation.
  */
 size_t dz_beam_select_workspace_bytes(int rows, int vocab, int k);
@@ -602,6 +602,7 @@ typedef struct dz_shared_attention_args {
 } dz_shared_attention_args;
 size_t dz_shared_attention_workspace_bytes(int num_seqs, int num_groups, int max_group, int max_shared, int max_keys, int q_heads,
                                            int kv_heads);
+int dz_shared_attention_max_seqs(void);
 int dz_shared_attention_decode(const dz_shared_attention_args* args, void* stream);
 
 /*
