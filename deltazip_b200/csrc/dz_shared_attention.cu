@@ -9,7 +9,7 @@
 // sequence's own keys for its query heads, and leaves a maximum, a sum and an unscaled output.  A second launch joins
 // them; nothing is counted or waited for between CTAs.
 //
-// One CTA of eight warps per SM stays for the whole launch.  It first lays out all parts (a scan over groups and
+// One CTA of twelve warps per SM stays for the whole launch.  It first lays out all parts (a scan over groups and
 // sequences in shared memory, the same in every CTA), then its warps take every n-th part: of shared keys in teams of
 // one, two or four warps with 16 rows each over the same key tiles, then of own keys each by itself.  A warp's ring of
 // key tiles runs on from part to part, so that the end of one is not waited for.  Neighbouring parts have
@@ -18,16 +18,18 @@
 // Rows are those of 16 x 8 x 16 warp MMAs.
 //   scores   S[16 rows, 8 keys] += Q K^T; the order of the 128 products of a score is free, so a lane's 16-byte piece of
 //            a key row serves two MMAs as it lies.
-//   output   O[16 rows, 128] += P V: a 32-bit weight is the sum of three 16-bit parts, all of its bits; the sums of the
-//            first part and of the other two are kept apart, so that an infinity in V, times a part that is zero, does not
-//            spoil the result.  V comes transposed by ldmatrix.
+//   output   O[16 rows, 128] += P V: a 32-bit weight is the sum of three 16-bit parts, all of its bits.  V comes
+//            transposed by ldmatrix.  Where V holds an infinity a part that is zero makes a NaN of it: a part of the
+//            keys whose output is not finite is summed again in plain 32-bit arithmetic, which few ever need.
+// A row's weights are taken relative to a maximum that moves only when it has grown by kSlack: moving it costs a
+// multiplication of the whole output, and among 16 rows one has a new maximum in nearly every tile.
 #include "dz_elem.cuh"
 
 namespace dz {
 namespace {
 
 constexpr int kDim = 128, kRows = 16;                          // rows of a warp
-constexpr int kWarps = 8, kThreads = kWarps * 32, kStages = 3, kTile = 16;     // keys per tile
+constexpr int kWarps = 12, kThreads = kWarps * 32, kStages = 2, kTile = 16;    // keys per tile
 constexpr int kRowBytes = kDim * 2, kHalfStage = kTile * kRowBytes, kStageBytes = 2 * kHalfStage;
 constexpr int kRingBytes = kStages * kStageBytes;
 constexpr int kMaxSeqs = 1536;           // also groups: what the layout of the parts takes of shared memory
@@ -43,6 +45,8 @@ struct SharedDecode {
   int64_t cache_rows;
   const int* tables;                     // [sequences, width]
   int width, block_size;
+  uint32_t block_magic;                  // key / block_size = key * block_magic >> block_shift
+  int block_shift;
   const int* lens;
   const int* starts;                     // [groups + 1]
   const int* shared;                     // [groups]
@@ -60,10 +64,11 @@ struct SharedDecode {
 // rows in eight different chunks.
 __device__ __forceinline__ int chunk_at(int r, int c) { return r * kRowBytes + ((c ^ ((r & 1) << 2 | (r >> 1 & 3))) << 4); }
 
-// Two weights in [0, 1] times `kScale` as three 16-bit numbers each (fp16: all bits of weights above 2^-16; below, what
-// is lost is at most 2^-40, which no sum of weights around 1 can hold).
+// Weights are at most 2^kSlack.  Two of them times `kScale` as three 16-bit numbers each (fp16: all bits of weights above
+// 2^-12; below, what is lost is at most 2^-36, which no sum of weights of 1 and more can hold).
+constexpr int kSlack = 4;
 template <typename T> constexpr float kScale = 1.f;
-template <> constexpr float kScale<__half> = 32768.f;
+template <> constexpr float kScale<__half> = 2048.f;
 template <typename T>
 __device__ __forceinline__ void split_weights(float a, float b, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
   a *= kScale<T>;
@@ -132,8 +137,37 @@ struct Part {
   int index;                             // among the parts of a row
 };
 
+__device__ __forceinline__ int64_t cache_row(const SharedDecode& p, int seq, int key) {
+  const int b = (int)((uint64_t)(uint32_t)key * p.block_magic >> p.block_shift);
+  const int64_t r = (int64_t)p.tables[(size_t)seq * p.width + b] * p.block_size + (key - b * p.block_size);
+  return min(max(r, (int64_t)0), p.cache_rows - 1);
+}
+
+// The output of one row over a part in plain arithmetic, a warp together: lane i has components 4 i ... 4 i + 3.
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(SharedDecode p) {
+__device__ __noinline__ float4 sum_plainly(const SharedDecode& p, Part part, int r, float m) {
+  const int lane = threadIdx.x & 31, ratio = p.heads / p.kv_heads;
+  auto four = [&](const T* from) {
+    const uint2 v = *reinterpret_cast<const uint2*>(from + lane * 4);
+    const float2 a = Cvt<T>::up(v.x), b = Cvt<T>::up(v.y);
+    return make_float4(a.x, a.y, b.x, b.y);
+  };
+  const float4 q = four((const T*)p.q + (size_t)(part.seq0 + r / ratio) * p.q_stride + (size_t)(part.kvh * ratio + r % ratio) * kDim);
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int key = part.t0; key < part.t1; ++key) {
+    const size_t at = (size_t)(cache_row(p, part.source, key) * p.kv_heads + part.kvh) * kDim;
+    const float4 k = four((const T*)p.k_cache + at), v = four((const T*)p.v_cache + at);
+    const float w = __expf(warp_sum(q.x * k.x + q.y * k.y + q.z * k.z + q.w * k.w) * p.scale - m);
+    o.x += w * v.x;
+    o.y += w * v.y;
+    o.z += w * v.z;
+    o.w += w * v.w;
+  }
+  return o;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid_constant__ SharedDecode p) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int s_warp[kWarps];
   int* s_starts = reinterpret_cast<int*>(smem + kWarps * kRingBytes);    // [groups + 1]
@@ -211,10 +245,8 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(SharedDecode
     int64_t row = 0;                                           // cache row of key 16 * tile + (lane & 15) of the next request
     auto find_row = [&]() {
       const int tile = ahead_step * team + member;
-      if (ahead_unit >= units || tile >= ahead.tiles) return;
-      const int k = min(ahead.t0 + tile * kTile + (lane & 15), ahead.t1 - 1), b = k / p.block_size;   // keys past the end repeat the last
-      const int64_t r = (int64_t)p.tables[(size_t)ahead.source * p.width + b] * p.block_size + (k - b * p.block_size);
-      row = min(max(r, (int64_t)0), p.cache_rows - 1);
+      if (ahead_unit < units && tile < ahead.tiles)            // keys past the end repeat the last
+        row = cache_row(p, ahead.source, min(ahead.t0 + tile * kTile + (lane & 15), ahead.t1 - 1));
     };
     auto request = [&](int to) {                               // and go on to the next one
       const int tile = ahead_step * team + member;
@@ -224,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(SharedDecode
 #pragma unroll
           for (int j = 0; j < kTile / 2; ++j) {
             const int r = 2 * j + (lane >> 4);
-            const int64_t from = (__shfl_sync(0xffffffffu, row, r) * p.kv_heads + ahead.kvh) * kDim + c * 8;
+            const int64_t from = __shfl_sync(0xffffffffu, (row * p.kv_heads + ahead.kvh) * kDim, r) + c * 8;
             uint8_t* dst = ring + to * kStageBytes + chunk_at(r, c);
             cp_async16(dst, kc + from, true);
             cp_async16(dst + kHalfStage, vc + from, r < keys);
@@ -258,11 +290,11 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(SharedDecode
           q[i][c] = r < part.rows ? *reinterpret_cast<const uint4*>(from + c * 32 + t * 8) : make_uint4(0, 0, 0, 0);
       }
       float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-      float o[16][4], o2[16][4];                               // [8 components][row gq: 2, row gq + 8: 2]: first parts, others
+      float o[16][4];                                          // [8 components][row gq: 2, row gq + 8: 2]
 #pragma unroll
       for (int j = 0; j < 16; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[j][e] = o2[j][e] = 0.f;
+        for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
 
       for (int step = 0; step * team < part.tiles; ++step) {
         cp_async_wait<kStages - 2>();
@@ -298,28 +330,28 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(SharedDecode
               for (int e = 0; e < 2; ++e)
                 if (k0 + i * 8 + 2 * t + e >= part.t1) x[i][0][e] = x[i][1][e] = -INFINITY;
           }
-          float ms[2], c[2];
+          float mx[2];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            float mx = fmaxf(fmaxf(x[0][h][0], x[0][h][1]), fmaxf(x[1][h][0], x[1][h][1]));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const float mn = fmaxf(m[h], mx);
-            ms[h] = mn == -INFINITY ? 0.f : mn;
-            c[h] = mn == m[h] ? 1.f : __expf(m[h] - ms[h]);
-            m[h] = mn;
+            mx[h] = fmaxf(fmaxf(x[0][h][0], x[0][h][1]), fmaxf(x[1][h][0], x[1][h][1]));
+            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
           }
-          if (__any_sync(0xffffffffu, c[0] != 1.f || c[1] != 1.f)) {
+          constexpr float kGrown = kSlack / kLog2e;
+          if (__any_sync(0xffffffffu, mx[0] > m[0] + kGrown || mx[1] > m[1] + kGrown)) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) l[h] *= c[h];
+            for (int h = 0; h < 2; ++h) {
+              const float mn = fmaxf(m[h], mx[h]), c = mn == m[h] ? 1.f : __expf(m[h] - mn);
+              m[h] = mn;
+              l[h] *= c;
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                o[j][e] *= c[e >> 1];
-                o2[j][e] *= c[e >> 1];
+              for (int j = 0; j < 16; ++j) {
+                o[j][2 * h] *= c;
+                o[j][2 * h + 1] *= c;
               }
+            }
           }
+          const float ms[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
           uint32_t hi[4], mid[4], low[4];
 #pragma unroll
           for (int i = 0; i < 2; ++i)
@@ -336,16 +368,15 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(SharedDecode
             ldsm4_t(b, vs + chunk_at(lane & 15, 2 * j + (lane >> 4)));
             mma16816<T>(o[2 * j], hi, b[0], b[1]);
             mma16816<T>(o[2 * j + 1], hi, b[2], b[3]);
-            mma16816<T>(o2[2 * j], mid, b[0], b[1]);
-            mma16816<T>(o2[2 * j + 1], mid, b[2], b[3]);
-            mma16816<T>(o2[2 * j], low, b[0], b[1]);
-            mma16816<T>(o2[2 * j + 1], low, b[2], b[3]);
+            mma16816<T>(o[2 * j], mid, b[0], b[1]);
+            mma16816<T>(o[2 * j + 1], mid, b[2], b[3]);
+            mma16816<T>(o[2 * j], low, b[0], b[1]);
+            mma16816<T>(o[2 * j + 1], low, b[2], b[3]);
           }
         }
         stage = stage == kStages - 1 ? 0 : stage + 1;
       }
-      // where the values held an infinity, the first parts' products are the result and the others' may be anything
-      auto whole = [](float a, float b) { return (isfinite(a) ? a + b : a) * (1.f / kScale<T>); };
+      bool finite = true;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
@@ -355,9 +386,22 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(SharedDecode
           const size_t to = ((size_t)seq * p.heads + part.kvh * ratio + r % ratio) * p.parts + part.index;
           float* out = p.partial + to * kDim + 2 * t;
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
-            *reinterpret_cast<float2*>(out + j * 8) = make_float2(whole(o[j][2 * h], o2[j][2 * h]), whole(o[j][2 * h + 1], o2[j][2 * h + 1]));
+          for (int j = 0; j < 16; ++j) {
+            finite = finite && isfinite(o[j][2 * h]) && isfinite(o[j][2 * h + 1]);
+            *reinterpret_cast<float2*>(out + j * 8) = make_float2(o[j][2 * h] * (1.f / kScale<T>), o[j][2 * h + 1] * (1.f / kScale<T>));
+          }
           if (t == 0) p.ml[to] = make_float2(m[h], l[h]);
+        }
+      }
+      if (__any_sync(0xffffffffu, !finite)) {
+        __syncwarp();
+        for (int i = 0; i < kRows; ++i) {
+          const int r = mine + i, seq = part.seq0 + r / ratio;
+          if (r >= part.rows || (!own && s_common[seq] == 0)) continue;
+          const float mr = __shfl_sync(0xffffffffu, i < 8 ? m[0] : m[1], (i & 7) * 4);
+          const size_t to = ((size_t)seq * p.heads + part.kvh * ratio + r % ratio) * p.parts + part.index;
+          const float4 v = sum_plainly<T>(p, part, r, mr);
+          *reinterpret_cast<float4*>(p.partial + to * kDim + lane * 4) = v;
         }
       }
     }
@@ -404,9 +448,9 @@ Plan plan(int num_seqs, int num_groups, int max_group, int max_shared, int max_k
   Plan r;
   const int64_t rows = (int64_t)(max_group < num_seqs ? max_group : num_seqs) * ratio;
   r.team = rows <= kRows ? 1 : rows <= 2 * kRows ? 2 : 4;
-  // about eight parts for every team, were all lengths two thirds of the longest; no more than a row's table takes
+  // about six parts for every team, were all lengths two thirds of the longest; no more than a row's table takes
   const int64_t keys = (num_groups * shared * ((rows + r.team * kRows - 1) / (r.team * kRows)) * r.team + num_seqs * (max_keys - shared)) * kv_heads * 2 / 3;
-  int64_t span = keys / (148 * kWarps * 8);
+  int64_t span = keys / (148 * kWarps * 6);
   const int64_t least = (max_keys + kMaxParts - 3) / (kMaxParts - 2);
   if (span < least) span = least;
   if (span < kMinSpan) span = kMinSpan;
@@ -462,10 +506,14 @@ int dz_shared_attention_decode(const dz_shared_attention_args* a, void* stream) 
                                                                                (int)keys, a->q_heads, a->kv_heads))
     return DZ_ERR_WORKSPACE;
   if (!aligned16(a->workspace)) return DZ_ERR_ALIGNMENT;
+  // floor(k / d) = k * ceil(2^(31 + l) / d) >> (31 + l) for k < 2^31, d <= 2^l
+  int log = 0;
+  while ((1ll << log) < a->block_size) ++log;
+  const uint32_t magic = (uint32_t)(((1ull << (31 + log)) + a->block_size - 1) / a->block_size);
   uint8_t* ws = reinterpret_cast<uint8_t*>(a->workspace);
   const Scratch at = scratch(a->num_seqs, a->q_heads, r);
   const SharedDecode p = {a->qkv, a->q_row_stride, a->out, a->k_cache, a->v_cache, a->cache_rows, a->block_tables, a->table_width,
-                          a->block_size, a->seq_lens, a->group_starts, a->shared_lens, a->num_groups, a->num_seqs, a->q_heads,
+                          a->block_size, magic, 31 + log, a->seq_lens, a->group_starts, a->shared_lens, a->num_groups, a->num_seqs, a->q_heads,
                           a->kv_heads, a->scale, a->max_group, a->max_shared, r.team, r.span, r.parts,
                           reinterpret_cast<float*>(ws), reinterpret_cast<float2*>(ws + at.ml), reinterpret_cast<int*>(ws + at.common)};
   cudaStream_t st = (cudaStream_t)stream;
