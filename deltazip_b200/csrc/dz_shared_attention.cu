@@ -42,7 +42,7 @@ struct SharedDecode {
   void* out;
   const void* k_cache;                   // [slots, kv_heads, 128]
   const void* v_cache;
-  int64_t cache_rows;
+  uint32_t last_row, last_page;          // of the cache
   const int* tables;                     // [sequences, width]
   int width, block_size;
   uint32_t block_magic;                  // key / block_size = key * block_magic >> block_shift
@@ -64,18 +64,23 @@ struct SharedDecode {
 // rows in eight different chunks.
 __device__ __forceinline__ int chunk_at(int r, int c) { return r * kRowBytes + ((c ^ ((r & 1) << 2 | (r >> 1 & 3))) << 4); }
 
-// Weights are at most 2^kSlack.  Two of them times `kScale` as three 16-bit numbers each (fp16: all bits of weights above
-// 2^-12; below, what is lost is at most 2^-36, which no sum of weights of 1 and more can hold).
+// Scores are kept times log2 e, and weights are 2^(score - maximum + kLift), at most 2^(kLift + kSlack).  Two of them as three
+// 16-bit numbers each: all bits (fp16: of weights above 2^-12 of the largest; below, what is lost is at most 2^-36 of it,
+// which no sum with the largest can hold).
 constexpr int kSlack = 4;
-template <typename T> constexpr float kScale = 1.f;
-template <> constexpr float kScale<__half> = 2048.f;
+template <typename T> constexpr int kLift = 0;
+template <> constexpr int kLift<__half> = 11;
 template <typename T>
 __device__ __forceinline__ void split_weights(float a, float b, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
-  a *= kScale<T>;
-  b *= kScale<T>;
   hi = Cvt<T>::down(a, b);
   const float2 h = Cvt<T>::up(hi);
   split_pair<T>(a - h.x, b - h.y, mid, lo);
+}
+
+__device__ __forceinline__ float exp2_of(float x) {            // (what is below 2^-126 is zero)
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 // How many keys a group shares, as far as they are read together.
@@ -100,6 +105,10 @@ __device__ __forceinline__ int common_keys(const SharedDecode& p, const int* sta
   if (first < 0 || seq < first || seq >= starts[g + 1] || seq - first >= p.max_group) return 0;
   const int n = shared_keys(p, g);
   return length_of(p, seq) >= n ? n : 0;
+}
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {      // the rest of 16 becomes zero
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
 // Running sums of count(i), i < n, in front of each i and at sums[n].  Every thread of the block calls it.
@@ -137,10 +146,11 @@ struct Part {
   int index;                             // among the parts of a row
 };
 
-__device__ __forceinline__ int64_t cache_row(const SharedDecode& p, int seq, int key) {
-  const int b = (int)((uint64_t)(uint32_t)key * p.block_magic >> p.block_shift);
-  const int64_t r = (int64_t)p.tables[(size_t)seq * p.width + b] * p.block_size + (key - b * p.block_size);
-  return min(max(r, (int64_t)0), p.cache_rows - 1);
+// The row of key `key` of the sequence with block table `table`, times heads: fits 32 bits (the host has looked).
+__device__ __forceinline__ uint32_t cache_row(const SharedDecode& p, const int* table, int key) {
+  const uint32_t b = (uint32_t)((uint64_t)(uint32_t)key * p.block_magic >> p.block_shift);
+  const uint32_t page = min((uint32_t)table[b], p.last_page);
+  return min(page * p.block_size + (key - b * p.block_size), p.last_row) * p.kv_heads;
 }
 
 // The output of one row over a part in plain arithmetic, a warp together: lane i has components 4 i ... 4 i + 3.
@@ -155,9 +165,9 @@ __device__ __noinline__ float4 sum_plainly(const SharedDecode& p, Part part, int
   const float4 q = four((const T*)p.q + (size_t)(part.seq0 + r / ratio) * p.q_stride + (size_t)(part.kvh * ratio + r % ratio) * kDim);
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int key = part.t0; key < part.t1; ++key) {
-    const size_t at = (size_t)(cache_row(p, part.source, key) * p.kv_heads + part.kvh) * kDim;
+    const size_t at = (size_t)(cache_row(p, p.tables + (size_t)part.source * p.width, key) + part.kvh) * kDim;
     const float4 k = four((const T*)p.k_cache + at), v = four((const T*)p.v_cache + at);
-    const float w = __expf(warp_sum(q.x * k.x + q.y * k.y + q.z * k.z + q.w * k.w) * p.scale - m);
+    const float w = exp2_of(warp_sum(q.x * k.x + q.y * k.y + q.z * k.z + q.w * k.w) * (p.scale * kLog2e) - m + kLift<T>);
     o.x += w * v.x;
     o.y += w * v.y;
     o.z += w * v.z;
@@ -200,8 +210,11 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid
   });
   __syncthreads();
 
-  const T* kc = (const T*)p.k_cache;
-  const T* vc = (const T*)p.v_cache;
+  uint8_t* const ring = smem + warp * kRingBytes;
+  const uint32_t ring_at = smem_addr(ring), lane_at = (uint32_t)chunk_at(lane >> 4, lane & 15);
+  const uint8_t* k_lane = (const uint8_t*)p.k_cache + (lane & 15) * 16;
+  const uint8_t* v_lane = (const uint8_t*)p.v_cache + (lane & 15) * 16;
+  const float scale = p.scale * kLog2e;
   for (int phase = 0; phase < 2; ++phase) {
     const bool own = phase == 1;
     const int team = own ? 1 : p.team, member = warp % team, first_warp = warp - member;
@@ -239,39 +252,43 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid
     };
 
     // The ring: what is requested runs kStages - 1 steps (a tile of every warp of the team) ahead of what is used.
-    uint8_t* ring = smem + warp * kRingBytes;
     int ahead_unit = unit, ahead_step = 0, stage = 0;
     Part ahead;
-    int64_t row = 0;                                           // cache row of key 16 * tile + (lane & 15) of the next request
+    const int* table = nullptr;
+    uint32_t row = 0;                                          // cache row and head of key 16 * tile + (lane & 15) of the next request
     auto find_row = [&]() {
       const int tile = ahead_step * team + member;
       if (ahead_unit < units && tile < ahead.tiles)            // keys past the end repeat the last
-        row = cache_row(p, ahead.source, min(ahead.t0 + tile * kTile + (lane & 15), ahead.t1 - 1));
+        row = cache_row(p, table, min(ahead.t0 + tile * kTile + (lane & 15), ahead.t1 - 1)) + ahead.kvh;
+    };
+    auto begin = [&]() {
+      if (ahead_unit >= units) return;
+      ahead = part_of(ahead_unit);
+      table = p.tables + (size_t)ahead.source * p.width;
     };
     auto request = [&](int to) {                               // and go on to the next one
       const int tile = ahead_step * team + member;
       if (ahead_unit < units) {
         if (tile < ahead.tiles) {
-          const int c = lane & 15, keys = ahead.t1 - ahead.t0 - tile * kTile;  // values past the end are zero, as their weights are
+          const int keys = ahead.t1 - ahead.t0 - tile * kTile; // values past the end are zero, as their weights are
 #pragma unroll
-          for (int j = 0; j < kTile / 2; ++j) {
-            const int r = 2 * j + (lane >> 4);
-            const int64_t from = __shfl_sync(0xffffffffu, (row * p.kv_heads + ahead.kvh) * kDim, r) + c * 8;
-            uint8_t* dst = ring + to * kStageBytes + chunk_at(r, c);
-            cp_async16(dst, kc + from, true);
-            cp_async16(dst + kHalfStage, vc + from, r < keys);
+          for (int j = 0; j < kTile / 2; ++j) {                // row 2 j + lane / 16, chunk lane % 16
+            const size_t from = (size_t)__shfl_sync(0xffffffffu, row, 2 * j + (lane >> 4)) * kRowBytes;
+            const uint32_t dst = ring_at + to * kStageBytes + (lane_at ^ (j & 3) << 4) + j * 2 * kRowBytes;
+            copy16(dst, k_lane + from, 16);
+            copy16(dst + kHalfStage, v_lane + from, 2 * j + (lane >> 4) < keys ? 16 : 0);
           }
         }
         if (++ahead_step * team >= ahead.tiles) {
           ahead_step = 0;
           ahead_unit += teams;
-          if (ahead_unit < units) ahead = part_of(ahead_unit);
+          begin();
         }
         find_row();
       }
       cp_async_commit();
     };
-    if (unit < units) ahead = part_of(unit);
+    begin();
     find_row();
 #pragma unroll
     for (int s = 0; s < kStages - 1; ++s) request(s);
@@ -307,22 +324,29 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid
           const uint8_t* ks = smem + (first_warp + w) * kRingBytes + stage * kStageBytes;
           const int k0 = part.t0 + tile * kTile;
           float x[2][2][2];                                    // [keys k0 + 8 i][row gq + 8 h][key 2 t + e]
+          // (products on one sum are kept apart: it takes some thirty cycles from one to the next)
+          float s[4][4];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+          for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const uint4 k = *reinterpret_cast<const uint4*>(ks + chunk_at(i * 8 + gq, 4 * c + t));
-              const uint32_t a0[4] = {q[0][c].x, q[1][c].x, q[0][c].y, q[1][c].y};
-              const uint32_t a1[4] = {q[0][c].z, q[1][c].z, q[0][c].w, q[1][c].w};
-              mma16816<T>(s[0], a0, k.x, k.y);
-              mma16816<T>(s[1], a1, k.z, k.w);
-            }
+            for (int e = 0; e < 4; ++e) s[i][e] = 0.f;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const uint4 ka = *reinterpret_cast<const uint4*>(ks + chunk_at(gq, 4 * c + t));
+            const uint4 kb = *reinterpret_cast<const uint4*>(ks + chunk_at(8 + gq, 4 * c + t));
+            const uint32_t a0[4] = {q[0][c].x, q[1][c].x, q[0][c].y, q[1][c].y};
+            const uint32_t a1[4] = {q[0][c].z, q[1][c].z, q[0][c].w, q[1][c].w};
+            mma16816<T>(s[0], a0, ka.x, ka.y);
+            mma16816<T>(s[1], a0, kb.x, kb.y);
+            mma16816<T>(s[2], a1, ka.z, ka.w);
+            mma16816<T>(s[3], a1, kb.z, kb.w);
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-              for (int e = 0; e < 2; ++e) x[i][h][e] = (s[0][2 * h + e] + s[1][2 * h + e]) * p.scale;
-          }
+              for (int e = 0; e < 2; ++e) x[i][h][e] = (s[i][2 * h + e] + s[2 + i][2 * h + e]) * scale;
           if (k0 + kTile > part.t1) {
 #pragma unroll
             for (int i = 0; i < 2; ++i)
@@ -337,11 +361,10 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid
             mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
             mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
           }
-          constexpr float kGrown = kSlack / kLog2e;
-          if (__any_sync(0xffffffffu, mx[0] > m[0] + kGrown || mx[1] > m[1] + kGrown)) {
+          if (__any_sync(0xffffffffu, mx[0] > m[0] + kSlack || mx[1] > m[1] + kSlack)) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const float mn = fmaxf(m[h], mx[h]), c = mn == m[h] ? 1.f : __expf(m[h] - mn);
+              const float mn = fmaxf(m[h], mx[h]), c = mn == m[h] ? 1.f : exp2_of(m[h] - mn);
               m[h] = mn;
               l[h] *= c;
 #pragma unroll
@@ -351,27 +374,31 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid
               }
             }
           }
-          const float ms[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+          const float ms[2] = {m[0] == -INFINITY ? 0.f : m[0] - kLift<T>, m[1] == -INFINITY ? 0.f : m[1] - kLift<T>};
           uint32_t hi[4], mid[4], low[4];
 #pragma unroll
           for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const float w0 = __expf(x[i][h][0] - ms[h]), w1 = __expf(x[i][h][1] - ms[h]);
+              const float w0 = exp2_of(x[i][h][0] - ms[h]), w1 = exp2_of(x[i][h][1] - ms[h]);
               l[h] += w0 + w1;
               split_weights<T>(w0, w1, hi[2 * i + h], mid[2 * i + h], low[2 * i + h]);
             }
           const uint8_t* vs = ks + kHalfStage;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            uint32_t b[4];
-            ldsm4_t(b, vs + chunk_at(lane & 15, 2 * j + (lane >> 4)));
-            mma16816<T>(o[2 * j], hi, b[0], b[1]);
-            mma16816<T>(o[2 * j + 1], hi, b[2], b[3]);
-            mma16816<T>(o[2 * j], mid, b[0], b[1]);
-            mma16816<T>(o[2 * j + 1], mid, b[2], b[3]);
-            mma16816<T>(o[2 * j], low, b[0], b[1]);
-            mma16816<T>(o[2 * j + 1], low, b[2], b[3]);
+          for (int j0 = 0; j0 < 8; j0 += 4) {
+            uint32_t b[4][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) ldsm4_t(b[j], vs + chunk_at(lane & 15, 2 * (j0 + j) + (lane >> 4)));
+#pragma unroll
+            for (int w = 0; w < 3; ++w) {
+              const uint32_t (&a)[4] = w == 0 ? hi : w == 1 ? mid : low;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                mma16816<T>(o[2 * (j0 + j)], a, b[j][0], b[j][1]);
+                mma16816<T>(o[2 * (j0 + j) + 1], a, b[j][2], b[j][3]);
+              }
+            }
           }
         }
         stage = stage == kStages - 1 ? 0 : stage + 1;
@@ -388,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
             finite = finite && isfinite(o[j][2 * h]) && isfinite(o[j][2 * h + 1]);
-            *reinterpret_cast<float2*>(out + j * 8) = make_float2(o[j][2 * h] * (1.f / kScale<T>), o[j][2 * h + 1] * (1.f / kScale<T>));
+            *reinterpret_cast<float2*>(out + j * 8) = make_float2(o[j][2 * h], o[j][2 * h + 1]);
           }
           if (t == 0) p.ml[to] = make_float2(m[h], l[h]);
         }
@@ -427,7 +454,7 @@ __global__ void __launch_bounds__(256) shared_join_kernel(SharedDecode p) {
   for (int i = 0; i < parts; ++i) {
     const float2 w = ml[i];
     const float4 v = *reinterpret_cast<const float4*>(from + (size_t)i * kDim);
-    const float c = w.x == -INFINITY ? 0.f : __expf(w.x - mm);
+    const float c = w.x == -INFINITY ? 0.f : exp2_of(w.x - mm);
     sum += w.y * c;
     a[0] += v.x * c;
     a[1] += v.y * c;
@@ -498,6 +525,7 @@ int dz_shared_attention_decode(const dz_shared_attention_args* a, void* stream) 
   if ((a->q_row_stride & 7) || !aligned16(a->qkv) || !aligned16(a->out) || !aligned16(a->k_cache) || !aligned16(a->v_cache))
     return DZ_ERR_ALIGNMENT;
   const int64_t keys = (int64_t)a->table_width * a->block_size;
+  if (a->cache_rows * a->kv_heads > 0x7fffffff || a->block_size > (1 << 30)) return DZ_ERR_TOO_LARGE;
   if (a->num_seqs > kMaxSeqs || a->num_groups > kMaxSeqs || keys > (1 << 30) || a->kv_heads > 4096) return DZ_ERR_TOO_LARGE;
   const Plan r = plan(a->num_seqs, a->num_groups, a->max_group, a->max_shared, (int)keys, a->q_heads, a->kv_heads);
   // parts are counted in 32 bits
@@ -512,7 +540,8 @@ int dz_shared_attention_decode(const dz_shared_attention_args* a, void* stream) 
   const uint32_t magic = (uint32_t)(((1ull << (31 + log)) + a->block_size - 1) / a->block_size);
   uint8_t* ws = reinterpret_cast<uint8_t*>(a->workspace);
   const Scratch at = scratch(a->num_seqs, a->q_heads, r);
-  const SharedDecode p = {a->qkv, a->q_row_stride, a->out, a->k_cache, a->v_cache, a->cache_rows, a->block_tables, a->table_width,
+  const SharedDecode p = {a->qkv, a->q_row_stride, a->out, a->k_cache, a->v_cache, (uint32_t)(a->cache_rows - 1),
+                          (uint32_t)((a->cache_rows - 1) / a->block_size), a->block_tables, a->table_width,
                           a->block_size, magic, 31 + log, a->seq_lens, a->group_starts, a->shared_lens, a->num_groups, a->num_seqs, a->q_heads,
                           a->kv_heads, a->scale, a->max_group, a->max_shared, r.team, r.span, r.parts,
                           reinterpret_cast<float*>(ws), reinterpret_cast<float2*>(ws + at.ml), reinterpret_cast<int*>(ws + at.common)};

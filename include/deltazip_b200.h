@@ -571,8 +571,8 @@ int dz_moe_gemm(const void* x, const void* weights, const int32_t* offsets, cons
  *                 group_starts[g + 1] (rising) have their first shared_lens[g] tokens in the same cache rows (their
  *                 tables begin alike), which are read once for the first max_group of them.  A sequence shorter than
  *                 that, or outside the groups, is read by itself; shared lengths above max_shared are read as
- *                 max_shared.  1 to 16 query heads per kv head.  A page number outside the cache is read as the
- *                 nearest row of it.  At most dz_shared_attention_max_seqs() sequences and groups.  The workspace (dz_shared_attention_workspace_bytes, max_keys = table_width *
+ *                 max_shared.  1 to 16 query heads per kv head.  A page number outside the cache is read as its
+ *                 last rows.  At most dz_shared_attention_max_seqs() sequences and groups.  The workspace (dz_shared_attention_workspace_bytes, max_keys = table_width *
  *                 block_size) needs no preparation.
  */
 size_t dz_beam_select_workspace_bytes(int rows, int vocab, int k);
