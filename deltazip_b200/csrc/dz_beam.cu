@@ -2,14 +2,17 @@
 // continuations, score[r, v] = c[r] + z[r, v] - log sum_v exp z[r, v], in one pass over the logits z.
 //
 // Within a row scores are in the order of the logits, so the k best of a group are among the k largest logits of each
-// piece of each of its rows.  Two launches:
-//   rows    a CTA takes a piece of a row into registers and leaves its maximum, its sum of exponentials and its k largest
-//           logits, sorted.  At least k logits reach the k-th largest of the maxima of 64 (k <= 32) or 256 groups of threads,
-//           and hardly more do: they are collected and ranked by counting.  Where many logits are equal (a mask) more
-//           may reach it than there is room for; then every thread names its best and the best of all is taken, k times.
-//   groups  a CTA joins its rows' maxima and sums and merges the pieces' lists: every thread holds the next entry of
-//           a list, and the best of all is taken, k times.
-// Sums are 32-bit inside a thread (at most 32 terms) and 64-bit beyond, and so are the scores that rows are compared by:
+// span of each of its rows.  Two launches:
+//   rows    a CTA goes through a span of a row a few thousand logits at a time, the next ones on their way, and leaves its
+//           maximum, its sum of exponentials and its k largest logits, sorted.  Of the first piece at least k logits reach the
+//           k-th largest of the maxima of 64 (k <= 32) or 256 groups of threads, and hardly more do; what reaches this
+//           floor is collected, ranked by counting and cut to the best k, and the floor rises.  Where many
+//           logits are equal (a mask) more may reach it than there is room for; then every thread names its best of
+//           the piece and the best of all is taken, k times.
+//   groups  a CTA joins its rows' maxima and sums, takes the entries of its spans' lists into registers, searches for a score
+//           that k to about 2 k of them reach, and ranks those by counting -- or, where too many are equal, takes the best
+//           one after the other.
+// Sums are 32-bit within a thread's piece (at most 32 terms) and 64-bit beyond, and so are the scores that rows are compared by:
 // beams come close to one another, and which is ahead is not to hang on a rounding.
 #include "dz_elem.cuh"
 
@@ -18,8 +21,8 @@ namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMaxKeep = 128;
-constexpr int kLarge = 32, kSmall = 8;   // elements of a thread
-constexpr int kRoom = 512;               // logits of a piece that are ranked by counting
+constexpr int kSmall = 8;                // elements of a thread and piece; larger pieces: 64 bytes
+constexpr int kRoom = 640;               // logits that are ranked by counting
 constexpr float kToLog2 = 1.4426950408889634f;                 // as a float, which is what the exponents are taken with
 constexpr double kLn2 = 0.6931471805599453;
 
@@ -72,168 +75,239 @@ __device__ __forceinline__ Key best_of_block(Key k, Key (*part)[kWarps], int tur
 struct BeamRows {
   const void* logits;
   int64_t stride;
-  int vocab, k, splits, width;           // width: entries of a list, k rounded up to four
+  int vocab, k, splits, pieces, width;   // pieces of a span; width: entries of a list, k rounded up to four
   double* sums;                          // [rows, splits] of 2^(z log2 e - ref)
   float2* tops;                          // maximum and ref
   float* values;                         // [rows, splits, width], best first
   int* tokens;                           // -1: none
 };
 
-// W elements are loaded at a time: 16 bytes where rows are aligned to that, else one.
-template <typename T, int E, int W>
+// The rank of found[i] among `n` in some threads' registers: `share` neighbouring threads count for one entry, and the first
+// of them calls use(entry, rank).  Every thread of the block calls it.
+template <typename F>
+__device__ __forceinline__ void rank_found(const uint64_t* found, int n, F use) {
+  const int share = n <= kThreads / 8 ? 8 : n <= kThreads / 4 ? 4 : n <= kThreads / 2 ? 2 : 1;
+  const int part = threadIdx.x & (share - 1);
+  for (int i0 = 0; i0 < n; i0 += kThreads / share) {
+    const int i = i0 + threadIdx.x / share;
+    const uint64_t key = found[min(i, n - 1)];
+    int rank = 0;
+#pragma unroll 4
+    for (int j = part; j < n; j += share) rank += found[j] > key;
+    for (int o = share >> 1; o > 0; o >>= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+    if (part == 0 && i < n) use(key, rank);
+  }
+}
+
+// A thread has E elements of a piece, in loads of 16 bytes: rows may start anywhere, so a row counts from the 16-byte boundary
+// at or before its first element, and what lies before it or behind its end is left out.
+template <typename T, int E>
 __global__ void __launch_bounds__(kThreads, 4) beam_rows_kernel(BeamRows p) {
-  constexpr int kPiece = kThreads * E;
-  __shared__ uint64_t s_found[kRoom];
-  __shared__ __align__(16) float s_max[kThreads];
+  constexpr int kPiece = kThreads * E, W = 16 / sizeof(T), kLoads = E / W;
+  extern __shared__ __align__(16) uint8_t s_ring[];            // two pieces
+  __shared__ uint64_t s_found[kRoom], s_best_k[kMaxKeep];
+  __shared__ __align__(16) uint32_t s_max[kThreads];
   __shared__ float s_floor, s_top[kWarps], s_ref[kWarps];
   __shared__ double s_sum[kWarps];
   __shared__ Key s_best[2][kWarps];
-  __shared__ int s_count;
+  __shared__ int s_new[3];
   const int row = blockIdx.y, split = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int base = split * kPiece, n = min(kPiece, p.vocab - base);
-  if (tid == 0) { s_count = 0; s_floor = -INFINITY; }
+  const T* start = (const T*)p.logits + (size_t)row * p.stride;
+  const int skip = (int)((uintptr_t)start & 15) / (int)sizeof(T);
+  const T* z = start - skip;                                   // 16-byte aligned
+  const int base = split * p.pieces * kPiece, end = min(base + p.pieces * kPiece, p.vocab + skip);
+  if (tid == 0) { s_new[0] = 0; s_floor = -INFINITY; }
   pdl_wait();
   pdl_launch();
-  const T* z = (const T*)p.logits + (size_t)row * p.stride + base;
-  // element j of a thread is at j / W * 256 W + tid W + j % W: rising with j.  What is behind the end counts as -inf.
+  // element j of a thread is at j / W * 256 W + tid W + j % W of the piece: rising with j.  A thread reads what it copied.
   auto place = [&](int j) { return j / W * (kThreads * W) + tid * W + j % W; };
-  float x[E];
+  auto load = [&](int from, int to) {
+    uint8_t* dst = s_ring + to * (kPiece * sizeof(T));
 #pragma unroll
-  for (int j = 0; j < E; j += W) {
-    const int at = place(j);
-    if constexpr (W > 1) {
-      if (at + W <= n) {
-        const uint4 v = __ldcs(reinterpret_cast<const uint4*>(z + at));
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    for (int j = 0; j < kLoads; ++j) {
+      const int at = from + place(j * W);
+      if (at < end) cp_async16(dst + (j * kThreads + tid) * 16, z + at, true);
+    }
+    cp_async_commit();
+  };
+  auto key_of = [](float v, int at) { return (uint64_t)ordered(v) << 32 | (0xffffffffu - (uint32_t)at); };
+  const bool few = p.k <= kThreads / 8;
+  const int groups = few ? kThreads / 4 : kThreads;
+  float top = -INFINITY, ref = -INFINITY;                      // of all the thread has seen
+  double total = 0.;                                           // relative to ref
+  int have = 0;                                                // collected
+  load(base, 0);
+  for (int piece = 0, from = base; from < end; ++piece, from += kPiece) {
+    load(from + kPiece, (piece + 1) & 1);
+    cp_async_wait<1>();
+    const uint8_t* ring = s_ring + (piece & 1) * (kPiece * sizeof(T));
+    float x[E];
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const uint4 v = *reinterpret_cast<const uint4*>(ring + (j * kThreads + tid) * 16);
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
         if constexpr (sizeof(T) == 4) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[j + e] = __uint_as_float(w[e]);
+          x[j * 4 + e] = __uint_as_float(w[e]);
         } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 f = Cvt<T>::up(w[e]);
-            x[j + 2 * e] = f.x;
-            x[j + 2 * e + 1] = f.y;
-          }
+          const float2 f = Cvt<T>::up(w[e]);
+          x[j * 8 + 2 * e] = f.x;
+          x[j * 8 + 2 * e + 1] = f.y;
         }
-        continue;
       }
     }
+    if (from < skip || from + kPiece > end) {                  // the row's first or last piece
 #pragma unroll
-    for (int e = 0; e < W; ++e) x[j + e] = at + e < n ? Cvt<T>::one(z[at + e]) : -INFINITY;
+      for (int j = 0; j < E; ++j)
+        if (from + place(j) < skip || from + place(j) >= end) x[j] = -INFINITY;
+    }
+    float eight[E / 8], mine = -INFINITY;                      // maxima of eight (fmaxf passes over NaN)
+#pragma unroll
+    for (int i = 0; i < E / 8; ++i) {
+      eight[i] = x[8 * i];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) eight[i] = fmaxf(eight[i], x[8 * i + j]);
+      mine = fmaxf(mine, eight[i]);
+    }
+    if (piece == 0) {
+      // the floor: the k-th largest maximum of the groups, less what the low bits hold instead: the group's number, so that
+      // no two are equal
+      if (few) {
+        float group = fmaxf(mine, __shfl_xor_sync(0xffffffffu, mine, 1));
+        group = fmaxf(group, __shfl_xor_sync(0xffffffffu, group, 2));
+        if ((lane & 3) == 0) s_max[tid >> 2] = ordered(group) & ~255u | tid;
+      } else {
+        s_max[tid] = ordered(mine) & ~255u | tid;
+      }
+      __syncthreads();
+      if (tid < groups) {
+        const uint32_t own = s_max[tid];
+        int rank = 0;
+#pragma unroll 8
+        for (int i = 0; i < groups; i += 4) {
+          const uint4 v = *reinterpret_cast<const uint4*>(s_max + i);
+          rank += (v.x > own) + (v.y > own) + (v.z > own) + (v.w > own);
+        }
+        if (rank == p.k - 1 && own >= ordered(-INFINITY) + 256) s_floor = unordered(own & ~255u);
+      }
+    }
+    // the sum, relative to the thread's own maximum: nothing is waited for
+    {
+      const float new_top = fmaxf(top, mine), new_ref = new_top * kToLog2;
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < E; ++j) sum += exp2_of(fmaf(x[j], kToLog2, -new_ref));
+      if (!(sum < INFINITY) || fabsf(new_ref) == INFINITY) {   // NaN, an infinity or very large logits among them
+        sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < E; ++j) sum += x[j] == new_top ? 1.f : x[j] < new_top ? exp2_of((x[j] - new_top) * kToLog2) : 0.f;
+        if (new_top == -INFINITY) sum = 0.f;
+      }
+      if (new_top != top) total *= weight_of(top, ref, new_top, new_ref);
+      total += sum;
+      top = new_top;
+      ref = new_ref;
+    }
+    if (piece == 0) __syncthreads();
+
+    // what reaches the floor
+    float floor_of = s_floor;
+    if (floor_of > -INFINITY) {
+      uint32_t reach = 0;
+      if (mine >= floor_of) {
+#pragma unroll
+        for (int i = 0; i < E / 8; ++i)
+          if (eight[i] >= floor_of) {
+#pragma unroll
+            for (int j = 8 * i; j < 8 * i + 8; ++j) reach |= x[j] >= floor_of ? 1u << j : 0u;
+          }
+        int at = have + atomicAdd(&s_new[piece % 3], __popc(reach));
+        for (; reach && at < kRoom; reach &= reach - 1) {      // few
+          const int i = place(__ffs(reach) - 1);
+          s_found[at++] = key_of(Cvt<T>::one(reinterpret_cast<const T*>(ring)[i]), from + i);
+        }
+      }
+    }
+    if (tid == 0) s_new[(piece + 1) % 3] = 0;
+    __syncthreads();
+    const int fresh = s_new[piece % 3];
+    bool cut = false;
+    if (floor_of > -INFINITY && have + fresh <= kRoom) {
+      have += fresh;
+      cut = have > p.k + p.k / 4;                              // (counting takes the square of it)
+    } else {
+      // more than there is room for, or hardly any above -inf: the best of what was kept and of the piece, one after the other
+      if (have > p.k) {                                        // (cut before)
+        rank_found(s_found, have, [&](uint64_t key, int rank) { if (rank < p.k) s_best_k[rank] = key; });
+        __syncthreads();
+        have = p.k;
+        if (tid < have) s_found[tid] = s_best_k[tid];
+        __syncthreads();
+      }
+      const uint64_t kept = tid < have ? s_found[tid] : 0;
+      uint64_t next = 0, last = ~0ull;
+      bool again = true;
+      int taken = 0;
+      for (; taken < p.k; ++taken) {
+        if (again) {                                           // the thread's best behind the last one taken
+          next = kept < last ? kept : 0;
+#pragma unroll
+          for (int j = 0; j < E; ++j) {
+            const int at = from + place(j);
+            const uint64_t key = key_of(fmaxf(x[j], -INFINITY), at);      // NaN counts as -inf
+            if (at >= skip && at < end && key < last && key > next) next = key;
+          }
+          again = false;
+        }
+        const Key best = best_of_block({next, (uint32_t)tid}, s_best, taken);
+        if (best.value == 0) break;
+        if (best.place == (uint32_t)tid) {
+          s_best_k[taken] = last = next;
+          again = true;
+        }
+      }
+      __syncthreads();
+      if (tid < taken) s_found[tid] = s_best_k[tid];
+      if (tid == 0) s_floor = taken == p.k ? unordered((uint32_t)(s_best_k[taken - 1] >> 32)) : -INFINITY;
+      have = taken;
+      __syncthreads();
+    }
+    if (cut && from + kPiece < end) {
+      rank_found(s_found, have, [&](uint64_t key, int rank) { if (rank < p.k) s_best_k[rank] = key; });
+      __syncthreads();
+      if (have > p.k) have = p.k;
+      if (tid < have) s_found[tid] = s_best_k[tid];
+      if (tid == 0 && have == p.k) s_floor = unordered((uint32_t)(s_best_k[have - 1] >> 32));
+      __syncthreads();
+    }
   }
-  float top = -INFINITY;                                       // (fmaxf passes over NaN)
-#pragma unroll
-  for (int j = 0; j < E; ++j) top = fmaxf(top, x[j]);
-  // the floor: the k-th largest maximum of 64 groups of four threads, or of all threads
-  const bool few = p.k <= kThreads / 8;
-  float group = top;
-  if (few) {
-    group = fmaxf(group, __shfl_xor_sync(0xffffffffu, group, 1));
-    group = fmaxf(group, __shfl_xor_sync(0xffffffffu, group, 2));
-    if ((lane & 3) == 0) s_max[tid >> 2] = group;
-  } else {
-    s_max[tid] = group;
-  }
-  // the sum relative to the thread's own maximum: nothing is waited for
-  float ref = top * kToLog2, sum = 0.f;
-#pragma unroll
-  for (int j = 0; j < E; ++j) sum += exp2_of(fmaf(x[j], kToLog2, -ref));
-  if (!(sum < INFINITY) || fabsf(ref) == INFINITY) {           // NaN, an infinity or very large logits among them
-    sum = 0.f;
-#pragma unroll
-    for (int j = 0; j < E; ++j) sum += x[j] == top ? 1.f : x[j] < top ? exp2_of((x[j] - top) * kToLog2) : 0.f;
-  }
-  if (top == -INFINITY) sum = 0.f;
+
   const float warp_top = warp_max(top), warp_ref = warp_max(ref);
-  double total = (double)sum * weight_of(top, ref, warp_top, warp_ref);
+  total *= weight_of(top, ref, warp_top, warp_ref);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   if (lane == 0) { s_top[warp] = warp_top; s_ref[warp] = warp_ref; s_sum[warp] = total; }
   __syncthreads();
-  const int groups = few ? kThreads / 4 : kThreads;
-  if (tid < groups) {
-    const float mine = s_max[tid];
-    int rank = 0;
-#pragma unroll 8
-    for (int i = 0; i < groups; i += 4) {
-      const float4 v = *reinterpret_cast<const float4*>(s_max + i);
-      rank += (v.x > mine || (v.x == mine && i < tid)) + (v.y > mine || (v.y == mine && i + 1 < tid)) +
-              (v.z > mine || (v.z == mine && i + 2 < tid)) + (v.w > mine || (v.w == mine && i + 3 < tid));
-    }
-    if (rank == p.k - 1) s_floor = mine;
-  }
-  const size_t piece = (size_t)row * p.splits + split;
-  if (warp == kWarps - 1) {                                    // meanwhile the sums of the warps
+  const size_t list = (size_t)row * p.splits + split;
+  if (warp == kWarps - 1) {
     const float m = lane < kWarps ? s_top[lane] : -INFINITY, r = lane < kWarps ? s_ref[lane] : -INFINITY;
     const float all_m = warp_max(m), all_r = warp_max(r);
     double t = lane < kWarps ? s_sum[lane] * weight_of(m, r, all_m, all_r) : 0.;
 #pragma unroll
     for (int o = 4; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
     if (lane == 0) {
-      p.sums[piece] = t;
-      p.tops[piece] = make_float2(all_m, all_r);
+      p.sums[list] = t;
+      p.tops[list] = make_float2(all_m, all_r);
     }
   }
-  __syncthreads();
-  const float floor_of = s_floor;
-  float* values = p.values + piece * p.width;
-  int* tokens = p.tokens + piece * p.width;
-  auto key_of = [&](int j) { return (uint64_t)ordered(x[j]) << 32 | (0xffffffffu - (uint32_t)place(j)); };
-  if (floor_of > -INFINITY) {
-    int first = 0, mine = 0;
-    if (top >= floor_of) {
-#pragma unroll
-      for (int j = 0; j < E; ++j) mine += x[j] >= floor_of;
-      first = atomicAdd(&s_count, mine);
-      if (first + mine <= kRoom) {
-#pragma unroll
-        for (int j = 0; j < E; ++j)
-          if (x[j] >= floor_of) s_found[first++] = key_of(j);
-      }
+  rank_found(s_found, have, [&](uint64_t key, int rank) {
+    if (rank < p.k) {
+      p.values[list * p.width + rank] = unordered((uint32_t)(key >> 32));
+      p.tokens[list * p.width + rank] = (int)(0xffffffffu - (uint32_t)key) - skip;
     }
-    __syncthreads();
-    const int count = s_count;
-    if (count <= kRoom) {
-      for (int i = tid; i < count; i += kThreads) {
-        const uint64_t key = s_found[i];
-        int rank = 0;
-#pragma unroll 4
-        for (int j = 0; j < count; ++j) rank += s_found[j] > key;
-        if (rank < p.k) {
-          values[rank] = unordered((uint32_t)(key >> 32));
-          tokens[rank] = base + (int)(0xffffffffu - (uint32_t)key);
-        }
-      }
-      return;
-    }
-  }
-  // many equal logits, or hardly any above -inf: one after the other
-  uint64_t next = 0, last = ~0ull;
-  bool fresh = true;
-  for (int i = 0; i < p.k; ++i) {
-    if (fresh) {                                               // the thread's best behind the last one taken
-      next = 0;
-#pragma unroll
-      for (int j = 0; j < E; ++j) {
-        x[j] = fmaxf(x[j], -INFINITY);                         // NaN counts as -inf
-        const uint64_t key = key_of(j);
-        if (place(j) < n && key < last && key > next) next = key;
-      }
-      fresh = false;
-    }
-    const Key best = best_of_block({next, (uint32_t)tid}, s_best, i);
-    if (best.value == 0) {
-      for (i += tid; i < p.k; i += kThreads) tokens[i] = -1;
-      break;
-    }
-    if (best.place == (uint32_t)tid) {
-      values[i] = unordered((uint32_t)(next >> 32));
-      tokens[i] = base + (int)(0xffffffffu - (uint32_t)next);
-      last = next;
-      fresh = true;
-    }
-  }
+  });
+  for (int i = have + tid; i < p.k; i += kThreads) p.tokens[list * p.width + i] = -1;
 }
 
 struct BeamGroups {
@@ -250,37 +324,48 @@ struct BeamGroups {
 };
 
 __global__ void __launch_bounds__(kThreads) beam_groups_kernel(BeamGroups p) {
-  constexpr int kLists = kThreads - 1;                        // one thread goes through what was kept of the lists before
-  __shared__ Key s_kept[2][kMaxKeep];                         // best first; place: entry of the group's lists
-  __shared__ int s_kept_token[2][kMaxKeep];
+  constexpr int kEntries = 8, kBatch = kThreads * kEntries;   // entries of the lists at a time
+  __shared__ Key s_kept[kMaxKeep], s_found[kRoom], s_best[2][kWarps];       // kept: best first; place: entry of the group's lists
+  __shared__ int s_kept_token[kMaxKeep], s_found_token[kRoom], s_count, s_part[2][kWarps];
   __shared__ double s_base[kThreads];                         // the score of a row's largest logit
   __shared__ float s_top[kThreads];                           // that logit (the lowest value of a type may be the largest: no sums with it)
   __shared__ uint8_t s_state[kThreads];                       // 0: none is possible, 1: as usual, 2: +inf alone
-  __shared__ Key s_best[2][kWarps];
   const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_wait();
   pdl_launch();
   const int first = min(max(p.starts[g], 0), p.rows), last = min(max(p.starts[g + 1], first), p.rows);
-  const int lists = (last - first) * p.splits;
-  int kept = 0, half = 0;
-  for (int l0 = 0; l0 < lists; l0 += kLists, half ^= 1) {
-    const int n = min(kLists, lists - l0), r0 = first + l0 / p.splits, r1 = first + (l0 + n - 1) / p.splits;
+  const int lists = (last - first) * p.splits, batch = min(kBatch / p.k, kThreads);      // lists at a time
+  int kept = 0;
+  for (int l0 = 0; l0 < lists; l0 += batch) {
+    const int n = min(batch, lists - l0), r0 = l0 / p.splits, r1 = (l0 + n - 1) / p.splits;
+    float value[kEntries];
+    int token[kEntries + 1];
+#pragma unroll
+    for (int j = 0; j < kEntries; ++j) {
+      const int e = j * kThreads + tid, l = e / p.k;
+      token[j] = -1;
+      value[j] = 0.f;
+      if (l < n) {
+        const size_t at = ((size_t)first * p.splits + l0 + l) * p.width + (e - l * p.k);
+        token[j] = p.tokens[at];
+        value[j] = p.values[at];
+      }
+    }
     __syncthreads();
+    if (tid == 0) s_count = 0;
     for (int r = r0 + warp; r <= r1; r += kWarps) {
-      const float c = p.scores[r];
+      const float c = p.scores[first + r];
+      const float2* tops = p.tops + (size_t)(first + r) * p.splits;
+      const double* sums = p.sums + (size_t)(first + r) * p.splits;
       float m = -INFINITY, ref = -INFINITY;
       for (int s = lane; s < p.splits; s += 32) {
-        const float2 t = p.tops[(size_t)r * p.splits + s];
-        m = fmaxf(m, t.x);
-        ref = fmaxf(ref, t.y);
+        m = fmaxf(m, tops[s].x);
+        ref = fmaxf(ref, tops[s].y);
       }
       m = warp_max(m);
       ref = warp_max(ref);
       double sum = 0.;
-      for (int s = lane; s < p.splits; s += 32) {
-        const float2 t = p.tops[(size_t)r * p.splits + s];
-        sum += p.sums[(size_t)r * p.splits + s] * weight_of(t.x, t.y, m, ref);
-      }
+      for (int s = lane; s < p.splits; s += 32) sum += sums[s] * weight_of(tops[s].x, tops[s].y, m, ref);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       if (lane == 0) {
@@ -293,94 +378,141 @@ __global__ void __launch_bounds__(kThreads) beam_groups_kernel(BeamGroups p) {
       }
     }
     __syncthreads();
-
-    // the thread's list: entries `at`, `at` + 1, ..., four of them at hand
-    Key mine = {0, 0xffffffffu};
-    int at = 0, token = -1, end = 0, state = 0;
-    uint32_t place0 = 0;
-    double base = 0.;
-    float top = 0.f;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    int4 t = make_int4(-1, -1, -1, -1);
-    const float* values = nullptr;
-    const int* tokens = nullptr;
-    if (tid < n) {
-      const int l = l0 + tid, r = first + l / p.splits;
-      state = s_state[r - r0];
-      base = s_base[r - r0];
-      top = s_top[r - r0];
-      place0 = (uint32_t)l * p.k;
-      values = p.values + ((size_t)first * p.splits + l) * p.width;
-      tokens = p.tokens + ((size_t)first * p.splits + l) * p.width;
-      // of a row where none is possible the first tokens, as all are equal
-      end = state != 0 ? p.k : l % p.splits == 0 ? min(p.k, p.vocab) : 0;
-    } else if (tid == kLists) {
-      end = kept;
-    }
-    auto fetch = [&]() {
-      mine = {0, 0xffffffffu};
-      if (at >= end) return;
-      if (tid == kLists) {
-        mine = s_kept[half ^ 1][at];
-        token = s_kept_token[half ^ 1][at];
-      } else if (state == 0) {
-        token = at;
-        mine = {ordered(-(double)INFINITY), place0 + at};
-      } else {
-        if (at % 4 == 0) {
-          v = *reinterpret_cast<const float4*>(values + at);
-          t = *reinterpret_cast<const int4*>(tokens + at);
-        } else {
-          v = make_float4(v.y, v.z, v.w, 0.f);
-          t = make_int4(t.y, t.z, t.w, -1);
-        }
-        token = t.x;
-        if (token < 0) { end = 0; return; }
+    Key key[kEntries + 1];
+    uint32_t largest = 0;
+    int real = 0;
+#pragma unroll
+    for (int j = 0; j < kEntries; ++j) {
+      const int e = j * kThreads + tid, l = e / p.k, i = e - l * p.k;
+      key[j] = {0, 0xffffffffu};
+      if (l < n) {
+        const int r = (l0 + l) / p.splits, state = s_state[r - r0];
         double s = -INFINITY;
-        if (state == 1) s = base + ((double)v.x - (double)top);
-        else if (v.x == INFINITY) s = base;
-        mine = {ordered(s), place0 + at};
-      }
-    };
-    fetch();
-    int taken = 0;
-    for (; taken < p.k; ++taken) {
-      const Key best = best_of_block(mine, s_best, taken);
-      if (best.value == 0) break;
-      if (mine.value == best.value && mine.place == best.place) {
-        s_kept[half][taken] = mine;
-        s_kept_token[half][taken] = token;
-        ++at;
-        fetch();
+        if (state == 0) token[j] = r * p.splits == l0 + l && i < p.vocab ? i : -1;       // the first tokens, as all are equal
+        else if (state == 1) s = s_base[r - r0] + ((double)value[j] - (double)s_top[r - r0]);
+        else if (value[j] == INFINITY) s = s_base[r - r0];
+        if (token[j] >= 0) key[j] = {ordered(s), (uint32_t)(l0 * p.k + e)};
       }
     }
-    kept = taken;
+    key[kEntries] = tid < kept ? s_kept[tid] : Key{0, 0xffffffffu};
+    token[kEntries] = tid < kept ? s_kept_token[tid] : -1;
+#pragma unroll
+    for (int j = 0; j <= kEntries; ++j) {
+      largest = max(largest, (uint32_t)(key[j].value >> 32));
+      real += key[j].value != 0;
+    }
+    // a floor for the upper halves of the keys: `lo` is reached by at least k (or is 0), `hi` by fewer
+    int turn = 0;
+    auto sum_of_block = [&](int x) {
+      x = __reduce_add_sync(0xffffffffu, x);
+      if (lane == 0) s_part[turn & 1][warp] = x;
+      __syncthreads();
+      x = __reduce_add_sync(0xffffffffu, lane < kWarps ? s_part[turn & 1][lane] : 0);
+      ++turn;
+      return x;
+    };
+    int count = sum_of_block(real);
+    uint32_t lo = 0;
+    if (count > 2 * p.k) {
+      largest = __reduce_max_sync(0xffffffffu, largest);
+      uint32_t hi = (uint32_t)(best_of_block({(uint64_t)largest << 32, 0}, s_best, 0).value >> 32) + 1;
+      while (count > 2 * p.k && hi - lo > 1) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        int reach = 0;
+#pragma unroll
+        for (int j = 0; j <= kEntries; ++j) reach += (uint32_t)(key[j].value >> 32) >= mid;
+        reach = sum_of_block(reach);
+        if (reach >= p.k) {
+          lo = mid;
+          count = reach;
+        } else {
+          hi = mid;
+        }
+      }
+    }
+    if (count <= kRoom) {
+#pragma unroll
+      for (int j = 0; j <= kEntries; ++j)
+        if (key[j].value != 0 && (uint32_t)(key[j].value >> 32) >= lo) {
+          const int at = atomicAdd(&s_count, 1);
+          s_found[at] = key[j];
+          s_found_token[at] = token[j];
+        }
+      __syncthreads();
+      const int share = count <= kThreads / 4 ? 4 : count <= kThreads / 2 ? 2 : 1;
+      for (int i0 = 0; i0 < count; i0 += kThreads / share) {
+        const int i = i0 + tid / share;
+        const Key k = s_found[min(i, count - 1)];
+        int rank = 0;
+#pragma unroll 4
+        for (int j = tid & (share - 1); j < count; j += share)
+          rank += s_found[j].value > k.value || (s_found[j].value == k.value && s_found[j].place < k.place);
+        for (int o = share >> 1; o > 0; o >>= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+        if ((tid & (share - 1)) == 0 && i < count && rank < p.k) {
+          s_kept[rank] = k;
+          s_kept_token[rank] = s_found_token[i];
+        }
+      }
+      kept = min(count, p.k);
+    } else {
+      for (kept = 0; kept < p.k; ++kept) {
+        Key best = key[0];
+        int best_token = token[0];
+#pragma unroll
+        for (int j = 1; j <= kEntries; ++j)
+          if (key[j].value > best.value || (key[j].value == best.value && key[j].place < best.place)) {
+            best = key[j];
+            best_token = token[j];
+          }
+        const Key taken = best_of_block(best, s_best, kept);   // (k of them are real: there are more than kRoom)
+        if (best.value == taken.value && best.place == taken.place) {
+          s_kept[kept] = best;
+          s_kept_token[kept] = best_token;
+#pragma unroll
+          for (int j = 0; j <= kEntries; ++j)
+            if (key[j].place == best.place) key[j].value = 0;
+        }
+      }
+    }
   }
   __syncthreads();
-  half ^= 1;
   for (int i = tid; i < p.k; i += kThreads) {
     const size_t at = (size_t)g * p.k + i;
     const bool real = i < kept;
-    p.out_scores[at] = real ? (float)unordered(s_kept[half][i].value) : -INFINITY;
-    p.out_rows[at] = real ? first + (int)(s_kept[half][i].place / (uint32_t)(p.splits * p.k)) : -1;
-    p.out_tokens[at] = real ? s_kept_token[half][i] : -1;
+    p.out_scores[at] = real ? (float)unordered(s_kept[i].value) : -INFINITY;
+    p.out_rows[at] = real ? first + (int)(s_kept[i].place / (uint32_t)(p.splits * p.k)) : -1;
+    p.out_tokens[at] = real ? s_kept_token[i] : -1;
   }
 }
 
-// Elements of a thread.  Small pieces spread few rows over the SMs.
-int elements(int rows, int vocab) { return (int64_t)rows * ((vocab + kThreads * kLarge - 1) / (kThreads * kLarge)) >= 148 ? kLarge : kSmall; }
-int pieces(int rows, int vocab) {
-  const int n = kThreads * elements(rows, vocab);
-  return (vocab + n - 1) / n;
+// How rows are cut: spans of pieces of `elements` per thread.  Small pieces, one a span, spread few rows over the SMs; where
+// there are enough of the large ones, spans are as long as four CTAs on every SM leave them.
+struct Cut {
+  int elements, pieces, splits;
+};
+Cut cut_rows(int rows, int vocab, int dtype) {
+  const int large = dtype == DZ_DTYPE_F32 ? 16 : 32, most = 148 * 4;
+  const int longest = vocab + 16 / (dtype == DZ_DTYPE_F32 ? 4 : 2) - 1;       // of a row counted from a 16-byte boundary
+  auto count = [&](int e) { return (longest + kThreads * e - 1) / (kThreads * e); };
+  Cut c = {large, 1, count(large)};
+  if ((int64_t)rows * c.splits < 148) {
+    c = {kSmall, 1, count(kSmall)};
+  } else {
+    const int want = (most + rows - 1) / rows;
+    if (want < c.splits) {
+      c.pieces = (c.splits + want - 1) / want;
+      c.splits = (c.splits + c.pieces - 1) / c.pieces;
+    }
+  }
+  return c;
 }
-
 int list_width(int k) { return (k + 3) / 4 * 4; }
 
 struct Scratch {
   size_t sums, tops, values, tokens, total;
 };
-Scratch scratch(int rows, int vocab, int k) {
-  const size_t n = (size_t)rows * pieces(rows, vocab), list = n * list_width(k) * 4;
+Scratch scratch(int rows, int splits, int k) {
+  const size_t n = (size_t)rows * splits, list = n * list_width(k) * 4;
   Scratch s;
   s.values = 0;
   s.tokens = list;
@@ -390,9 +522,10 @@ Scratch scratch(int rows, int vocab, int k) {
   return s;
 }
 
-template <typename T, int E, int W>
+template <typename T, int E>
 int launch_rows(const BeamRows& p, int rows, cudaStream_t st) {
-  DZ_CUDA_OK(launch_pdl(beam_rows_kernel<T, E, W>, dim3(p.splits, rows), dim3(kThreads), st, p));
+  const size_t smem = 2 * kThreads * E * sizeof(T);
+  DZ_CUDA_OK(launch_ex(beam_rows_kernel<T, E>, dim3(p.splits, rows), dim3(kThreads), smem, 1, st, p));
   return DZ_OK;
 }
 
@@ -405,7 +538,12 @@ extern "C" {
 
 size_t dz_beam_select_workspace_bytes(int rows, int vocab, int k) {
   if (rows <= 0 || vocab <= 0 || k <= 0 || k > kMaxKeep) return 0;
-  return scratch(rows, vocab, k).total;
+  size_t most = 0;                                             // whatever the type
+  for (int dtype : {DZ_DTYPE_F16, DZ_DTYPE_F32}) {
+    const size_t n = scratch(rows, cut_rows(rows, vocab, dtype).splits, k).total;
+    if (n > most) most = n;
+  }
+  return most;
 }
 
 int dz_beam_select(const void* logits, int64_t row_stride, int rows, int vocab, const float* scores, const int32_t* group_starts,
@@ -418,21 +556,19 @@ int dz_beam_select(const void* logits, int64_t row_stride, int rows, int vocab, 
   if (k > kMaxKeep || rows > 65535 || vocab > (1 << 30)) return DZ_ERR_TOO_LARGE;
   const int size = dtype == DZ_DTYPE_F32 ? 4 : 2;
   if ((uintptr_t)logits % size) return DZ_ERR_ALIGNMENT;
-  const int splits = rows > 0 ? pieces(rows, vocab) : 1;
+  const Cut cut = cut_rows(rows > 0 ? rows : 1, vocab, dtype);
+  const int splits = cut.splits;
   if ((int64_t)rows * splits * k > 0x7fffffff) return DZ_ERR_TOO_LARGE;
   uint8_t* ws = (uint8_t*)workspace;
-  const Scratch at = scratch(rows, vocab, k);
+  const Scratch at = scratch(rows, splits, k);
   cudaStream_t st = (cudaStream_t)stream;
   if (rows > 0) {
     if (!ws || workspace_bytes < at.total) return DZ_ERR_WORKSPACE;
     if (!aligned16(ws)) return DZ_ERR_ALIGNMENT;
-    const BeamRows p = {logits, row_stride, vocab, k, splits, list_width(k), (double*)(ws + at.sums), (float2*)(ws + at.tops),
+    const BeamRows p = {logits, row_stride, vocab, k, splits, cut.pieces, list_width(k), (double*)(ws + at.sums), (float2*)(ws + at.tops),
                         (float*)(ws + at.values), (int*)(ws + at.tokens)};
-    const bool wide = aligned16(logits) && (rows == 1 || row_stride * size % 16 == 0), large = elements(rows, vocab) == kLarge;
     int rc = DZ_OK;
-    DZ_DISPATCH(dtype, constexpr int W = 16 / sizeof(T);
-                rc = large ? (wide ? launch_rows<T, kLarge, W>(p, rows, st) : launch_rows<T, kLarge, 1>(p, rows, st))
-                           : (wide ? launch_rows<T, kSmall, W>(p, rows, st) : launch_rows<T, kSmall, 1>(p, rows, st)));
+    DZ_DISPATCH(dtype, rc = cut.elements == kSmall ? launch_rows<T, kSmall>(p, rows, st) : launch_rows<T, 64 / sizeof(T)>(p, rows, st));
     if (rc != DZ_OK) return rc;
   }
   const BeamGroups q = {group_starts, scores, (const double*)(ws + at.sums), (const float2*)(ws + at.tops),
