@@ -216,7 +216,7 @@ _SIGNATURES = {
     "dz_beam_select": (c_int, [c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p,
                                c_void_p, c_size_t, c_int, c_void_p]),
     "dz_copy_pages_max_pairs": (c_int, []),
-    "dz_copy_pages": (c_int, [c_void_p, c_int, c_int, c_int, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
+    "dz_copy_pages": (c_int, [c_void_p, c_int, c_int, c_int, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
     "dz_shared_attention_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
     "dz_shared_attention_max_seqs": (c_int, []),
     "dz_shared_attention_decode": (c_int, [POINTER(SharedAttentionArgs), c_void_p]),

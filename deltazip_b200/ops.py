@@ -998,16 +998,27 @@ def mlstm(x: torch.Tensor, h: torch.Tensor, w_if: torch.Tensor, b_if: torch.Tens
 
 def _need_here(*tensors) -> None:
     """CUDA tensors of the current device, on whose stream the work is enqueued."""
-    _need_cuda(*tensors)
     here = torch._C._cuda_getDevice()
     for t in tensors:
-        if t is not None and t.device.index != here:
-            raise ValueError(f"a tensor is on GPU {t.device.index}, the current one is {here}")
+        if t is not None and t.get_device() != here:
+            _need_cuda(t)
+            raise ValueError(f"a tensor is on GPU {t.get_device()}, the current one is {here}")
 
 
 def _need_int32(what: str, *tensors) -> None:
-    if any(t is not None and (t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous()) for t in tensors):
-        raise ValueError(f"{what} must be contiguous int32 vectors")
+    for t in tensors:
+        if t is not None and (t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous()):
+            raise ValueError(f"{what} must be contiguous int32 vectors")
+
+
+@functools.lru_cache(maxsize=4096)
+def _beam_workspace_bytes(rows: int, vocab: int, k: int) -> int:
+    return lib().dz_beam_select_workspace_bytes(rows, vocab, k)
+
+
+@functools.lru_cache(maxsize=4096)
+def _shared_workspace_bytes(*sizes: int) -> int:
+    return lib().dz_shared_attention_workspace_bytes(*sizes)
 
 
 class BeamCandidates(NamedTuple):
@@ -1035,11 +1046,13 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, group_starts: torch.
     stride = logits.stride(0) if rows > 1 else vocab
     out = torch.empty((3, groups, max(k, 0)), dtype=torch.int32, device=logits.device)
     # fresh scratch for every call: two captured graphs never share it
-    ws = torch.empty(lib().dz_beam_select_workspace_bytes(rows, vocab, k), dtype=torch.uint8, device=logits.device)
+    size = _beam_workspace_bytes(rows, vocab, k)
+    ws = torch.empty(size, dtype=torch.uint8, device=logits.device)
+    to, step = out.data_ptr(), 4 * groups * k
     check(lib().dz_beam_select(logits.data_ptr(), stride, rows, vocab, scores.data_ptr(), group_starts.data_ptr(), groups, k,
-                               out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), ws.data_ptr(), ws.numel(), code,
-                               _stream()), "dz_beam_select")
-    return BeamCandidates(out[0].view(torch.float32), out[1], out[2])
+                               to, to + step, to + 2 * step, ws.data_ptr(), size, code, _stream()), "dz_beam_select")
+    best, row, token = out.unbind()
+    return BeamCandidates(best.view(torch.float32), row, token)
 
 
 class PagePools:
@@ -1065,6 +1078,7 @@ class PagePools:
             unit = next(u for u in (16, 8, 4, 2, 1) if row % u == 0 and t.data_ptr() % u == 0)
             entries.append([t.data_ptr(), row, self.rows_per_page, unit])
             self.page_units += row // unit * self.rows_per_page
+        self.alike = int(len({(row, unit) for _, row, _, unit in entries}) == 1)
         self.device = self.tensors[0].device if self.tensors else None
         self.table = torch.tensor(entries, dtype=torch.int64).to(self.device) if entries else None
 
@@ -1082,7 +1096,7 @@ def copy_pages(pools: PagePools, src: torch.Tensor, dst: torch.Tensor, rows: Opt
         return
     _need_here(pools.table)
     check(lib().dz_copy_pages(pools.table.data_ptr(), len(pools.tensors), pools.num_pages, pools.rows_per_page, pools.page_units,
-                              src.data_ptr(), dst.data_ptr(), _ptr(rows), src.numel(), _stream()), "dz_copy_pages")
+                              pools.alike, src.data_ptr(), dst.data_ptr(), _ptr(rows), src.numel(), _stream()), "dz_copy_pages")
 
 
 def copy_pages_max_pairs() -> int:
@@ -1112,22 +1126,21 @@ def shared_attention_decode(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: t
         raise ValueError("block_tables [B, pages] and seq_lens [B] must be contiguous int32")
     if shared_lens.numel() != max(0, group_starts.numel() - 1):
         raise ValueError("group_starts has one entry more than shared_lens")
-    for cache in (k_cache, v_cache):
-        if cache.dim() != 3 or tuple(cache.shape[1:]) != (kv_heads, 128) or cache.dtype != qkv.dtype or not cache.is_contiguous():
-            raise ValueError(f"the caches must be contiguous [slots, {kv_heads}, 128] of the queries' type")
-    if k_cache.shape != v_cache.shape:
-        raise ValueError("the caches of keys and values have the same slots")
+    shape = k_cache.shape
+    if shape != v_cache.shape or shape[1:] != (kv_heads, 128) or k_cache.dtype is not qkv.dtype or \
+            v_cache.dtype is not qkv.dtype or not k_cache.is_contiguous() or not v_cache.is_contiguous():
+        raise ValueError(f"the caches must be contiguous [slots, {kv_heads}, 128] of the queries' type")
     if out is None:
         out = torch.empty((b, q_heads * 128), dtype=qkv.dtype, device=qkv.device)
     elif out.shape != (b, q_heads * 128) or out.dtype != qkv.dtype or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous [{b}, {q_heads * 128}] of the queries' type")
     groups, keys = shared_lens.numel(), block_tables.shape[1] * block_size
-    ws = torch.empty(lib().dz_shared_attention_workspace_bytes(b, groups, max_group, max_shared, keys, q_heads, kv_heads),
-                     dtype=torch.uint8, device=qkv.device)
+    size = _shared_workspace_bytes(b, groups, max_group, max_shared, keys, q_heads, kv_heads)
+    ws = torch.empty(size, dtype=torch.uint8, device=qkv.device)
     args = _lib.SharedAttentionArgs(
         qkv.data_ptr(), qkv.stride(0) if b > 1 else width, out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0],
         block_tables.data_ptr(), block_tables.shape[1], block_size, seq_lens.data_ptr(), group_starts.data_ptr(),
-        shared_lens.data_ptr(), groups, b, max_group, max_shared, q_heads, kv_heads, 128, float(scale), ws.data_ptr(), ws.numel(),
+        shared_lens.data_ptr(), groups, b, max_group, max_shared, q_heads, kv_heads, 128, float(scale), ws.data_ptr(), size,
         _dtype_code(qkv))
     check(lib().dz_shared_attention_decode(ctypes.byref(args), _stream()), "dz_shared_attention_decode")
     return out

@@ -565,7 +565,8 @@ int dz_moe_gemm(const void* x, const void* weights, const int32_t* offsets, cons
  *                 pages of page_rows rows.  For pairs (src, dst, rows) the first rows (NULL: all) of page dst become
  *                 what those of page src were before the call, in every pool.  A page may be source and destination;
  *                 of several pairs with one destination the last counts; pairs with a page outside [0, num_pages) are
- *                 left out.  page_units: units of a page in all pools together.  At most dz_copy_pages_max_pairs() pairs.
+ *                 left out.  page_units: units of a page in all pools together; alike: whether all pools have the same
+ *                 row bytes and unit.  At most dz_copy_pages_max_pairs() pairs.
  *   shared_attention_decode
  *                 dz_paged_attention_decode for sequences in groups: sequences group_starts[g] <= s <
  *                 group_starts[g + 1] (rising) have their first shared_lens[g] tokens in the same cache rows (their
@@ -580,8 +581,8 @@ int dz_beam_select(const void* logits, int64_t row_stride, int rows, int vocab, 
                    int num_groups, int k, float* out_scores, int32_t* out_rows, int32_t* out_tokens, void* workspace,
                    size_t workspace_bytes, int dtype, void* stream);
 int dz_copy_pages_max_pairs(void);
-int dz_copy_pages(const int64_t* pools, int num_pools, int num_pages, int page_rows, int64_t page_units, const int32_t* src,
-                  const int32_t* dst, const int32_t* rows, int pairs, void* stream);
+int dz_copy_pages(const int64_t* pools, int num_pools, int num_pages, int page_rows, int64_t page_units, int alike,
+                  const int32_t* src, const int32_t* dst, const int32_t* rows, int pairs, void* stream);
 typedef struct dz_shared_attention_args {
   const void* qkv;
   int64_t q_row_stride;
