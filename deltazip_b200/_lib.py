@@ -127,6 +127,7 @@ class SharedAttentionArgs(Structure):
         ("seq_lens", c_void_p), ("group_starts", c_void_p), ("shared_lens", c_void_p), ("num_groups", c_int32),
         ("num_seqs", c_int32), ("max_group", c_int32), ("max_shared", c_int32), ("q_heads", c_int32), ("kv_heads", c_int32),
         ("head_dim", c_int32), ("scale", c_float), ("workspace", c_void_p), ("workspace_bytes", c_size_t), ("dtype", c_int32),
+        ("status", c_void_p),
     ]
 
 

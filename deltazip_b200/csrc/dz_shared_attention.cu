@@ -9,21 +9,28 @@
 // sequence's own keys for its query heads, and leaves a maximum, a sum and an unscaled output.  A second launch joins
 // them; nothing is counted or waited for between CTAs.
 //
-// One CTA of twelve warps per SM stays for the whole launch.  It first lays out all parts (a scan over groups and
-// sequences in shared memory, the same in every CTA), then its warps take every n-th part: of shared keys in teams of
-// one, two or four warps with 16 rows each over the same key tiles, then of own keys each by itself.  A warp's ring of
-// key tiles runs on from part to part, so that the end of one is not waited for.  Neighbouring parts have
+// One CTA of twelve warps per SM stays for the whole launch.  It first lays out all parts (how long they are and how many,
+// by scans over groups and sequences in shared memory, the same in every CTA), then its warps take every n-th part: of shared
+// keys in teams of one, two or four warps with 16 rows each over the same key tiles, then of own keys each by itself.  A
+// warp's ring of key tiles runs on from part to part, so that the end of one is not waited for.  Neighbouring parts have
 // neighbouring heads of the same cache rows, and go to different SMs.
 //
+// Tiles are 16 keys that begin at a multiple of 16.  Where pages are whole tiles, a tile is four TMA boxes of 16 rows x 128
+// bytes; otherwise each row is copied by itself.
+//
 // Rows are those of 16 x 8 x 16 warp MMAs.
-//   scores   S[16 rows, 8 keys] += Q K^T; the order of the 128 products of a score is free, so a lane's 16-byte piece of
+//   scores   S[rows, 8 keys] += Q K^T; the order of the 128 products of a score is free, so a lane's 16-byte piece of
 //            a key row serves two MMAs as it lies.
-//   output   O[16 rows, 128] += P V: a 32-bit weight is the sum of three 16-bit parts, all of its bits.  V comes
-//            transposed by ldmatrix.  Where V holds an infinity a part that is zero makes a NaN of it: a part of the
-//            keys whose output is not finite is summed again in plain 32-bit arithmetic, which few ever need.
+//   output   O[rows, 128] += P V: a 32-bit weight is the sum of three 16-bit parts, all of its bits.  V comes
+//            transposed by ldmatrix.
+// With up to eight rows the other eight of an MMA carry the second and third parts: two MMAs of half the first part each,
+// one with the second and one with the third beside it, 48 MMAs a tile instead of 64; and an infinity in V is found in the
+// first part's sums.  With more rows, where a part of a weight that is zero makes a NaN of an infinity, output that is
+// not finite is summed again in plain 32-bit arithmetic, which few ever need.
 // A row's weights are taken relative to a maximum that moves only when it has grown by kSlack: moving it costs a
 // multiplication of the whole output, and among 16 rows one has a new maximum in nearly every tile.
 #include "dz_elem.cuh"
+#include "dz_tc.cuh"
 
 namespace dz {
 namespace {
@@ -34,7 +41,7 @@ constexpr int kRowBytes = kDim * 2, kHalfStage = kTile * kRowBytes, kStageBytes 
 constexpr int kRingBytes = kStages * kStageBytes;
 constexpr int kMaxSeqs = 1536;           // also groups: what the layout of the parts takes of shared memory
 constexpr int kMaxParts = 64;            // of a row
-constexpr int kMinSpan = 64;             // keys of a part: a step of four warps
+constexpr int kEight = 8;                // rows that leave half of an MMA's to the weights' parts
 
 struct SharedDecode {
   const void* q;
@@ -54,15 +61,19 @@ struct SharedDecode {
   float scale;
   int max_group, max_shared;
   int team;                              // warps that take shared keys together (1, 2, 4)
-  int span, parts;                       // keys of a part; parts of a row at most
+  int least, parts;                      // keys of a part at least, parts of a row at most
   float* partial;                        // [sequences, heads, parts, 128]
   float2* ml;                            // [sequences, heads, parts] maximum and sum
   int* common;                           // [sequences] keys that a sequence reads with its group
+  int* spans;                            // [2] keys of a part of shared and of own keys
+  int* status;
 };
 
-// Where 16-byte chunk c of row r lies: rows r, r + 1 in different halves of the banks, any eight consecutive
-// rows in eight different chunks.
-__device__ __forceinline__ int chunk_at(int r, int c) { return r * kRowBytes + ((c ^ ((r & 1) << 2 | (r >> 1 & 3))) << 4); }
+// Where 16-byte chunk c of row r of 16 lies: two halves of 128 bytes a row, chunks of a half in the order of TMA's 128-byte
+// swizzle, so that neither the 16-byte reads of K nor ldmatrix meet a bank twice.
+__device__ __forceinline__ int chunk_at(int r, int c) { return (c >> 3) * (kHalfStage / 2) + r * 128 + (((c ^ r) & 7) << 4); }
+// The chunk of K and Q that a lane (t = lane % 4) has of the c-th quarter.
+__device__ __forceinline__ int quarter(int c, int t) { return (c >> 1) * 8 + 2 * t + (c & 1); }
 
 // Scores are kept times log2 e, and weights are 2^(score - maximum + kLift), at most 2^(kLift + kSlack).  Two of them as three
 // 16-bit numbers each: all bits (fp16: of weights above 2^-12 of the largest; below, what is lost is at most 2^-36 of it,
@@ -71,10 +82,10 @@ constexpr int kSlack = 4;
 template <typename T> constexpr int kLift = 0;
 template <> constexpr int kLift<__half> = 11;
 template <typename T>
-__device__ __forceinline__ void split_weights(float a, float b, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
+__device__ __forceinline__ void split_weights(float a, float b, float times, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
   hi = Cvt<T>::down(a, b);
   const float2 h = Cvt<T>::up(hi);
-  split_pair<T>(a - h.x, b - h.y, mid, lo);
+  split_pair<T>(times * (a - h.x), times * (b - h.y), mid, lo);    // of what the first part leaves, `times` over
 }
 
 __device__ __forceinline__ float exp2_of(float x) {            // (what is below 2^-126 is zero)
@@ -111,7 +122,20 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes)
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
-// Running sums of count(i), i < n, in front of each i and at sums[n].  Every thread of the block calls it.
+__device__ __forceinline__ int64_t sum_of_block(int64_t x, int64_t* part) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = x;
+  __syncthreads();
+  x = 0;
+  for (int w = 0; w < kWarps; ++w) x += part[w];
+  __syncthreads();
+  return x;
+}
+
+// Running sums of count(i), i < n, in front of each i and at sums[n]; count may read sums[i].  Every thread of the block
+// calls it.
 template <typename F>
 __device__ __forceinline__ void lay_out(int n, int* sums, int* warp_sums, F count) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -138,19 +162,19 @@ __device__ __forceinline__ void lay_out(int n, int* sums, int* warp_sums, F coun
   if (threadIdx.x == 0) sums[n] = before;
 }
 
-// A span of keys for some rows.
+// A span of keys for some rows: tiles from t0 on, of which the keys t_lo <= t < t1 count.
 struct Part {
-  int kvh, t0, t1, tiles;
+  int kvh, t0, t_lo, t1, tiles;
   int source;                            // the sequence in whose table the keys are
   int seq0, row0, rows;                  // rows (seq0 + r / ratio, kvh * ratio + r % ratio), row0 <= r < rows
   int index;                             // among the parts of a row
 };
 
-// The row of key `key` of the sequence with block table `table`, times heads: fits 32 bits (the host has looked).
+// The cache row of key `key` of the sequence with block table `table`; times heads it fits 32 bits (the host has looked).
 __device__ __forceinline__ uint32_t cache_row(const SharedDecode& p, const int* table, int key) {
   const uint32_t b = (uint32_t)((uint64_t)(uint32_t)key * p.block_magic >> p.block_shift);
   const uint32_t page = min((uint32_t)table[b], p.last_page);
-  return min(page * p.block_size + (key - b * p.block_size), p.last_row) * p.kv_heads;
+  return min(page * p.block_size + (key - b * p.block_size), p.last_row);
 }
 
 // The output of one row over a part in plain arithmetic, a warp together: lane i has components 4 i ... 4 i + 3.
@@ -164,8 +188,8 @@ __device__ __noinline__ float4 sum_plainly(const SharedDecode& p, Part part, int
   };
   const float4 q = four((const T*)p.q + (size_t)(part.seq0 + r / ratio) * p.q_stride + (size_t)(part.kvh * ratio + r % ratio) * kDim);
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int key = part.t0; key < part.t1; ++key) {
-    const size_t at = (size_t)(cache_row(p, p.tables + (size_t)part.source * p.width, key) + part.kvh) * kDim;
+  for (int key = part.t_lo; key < part.t1; ++key) {
+    const size_t at = ((size_t)cache_row(p, p.tables + (size_t)part.source * p.width, key) * p.kv_heads + part.kvh) * kDim;
     const float4 k = four((const T*)p.k_cache + at), v = four((const T*)p.v_cache + at);
     const float w = exp2_of(warp_sum(q.x * k.x + q.y * k.y + q.z * k.z + q.w * k.w) * (p.scale * kLog2e) - m + kLift<T>);
     o.x += w * v.x;
@@ -176,265 +200,408 @@ __device__ __noinline__ float4 sum_plainly(const SharedDecode& p, Part part, int
   return o;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 1) shared_decode_kernel(const __grid_constant__ SharedDecode p) {
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int s_warp[kWarps];
-  int* s_starts = reinterpret_cast<int*>(smem + kWarps * kRingBytes);    // [groups + 1]
-  int* s_source = s_starts + p.groups + 1;                    // [groups] first sequence that has all the shared keys
-  int* s_shared = s_source + p.groups;                        // [groups + 1] parts of shared keys, over heads
-  int* s_common = s_shared + p.groups + 1;                    // [sequences]
-  int* s_own = s_common + p.seqs;                             // [sequences + 1] parts of own keys
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gq = lane >> 2, t = lane & 3;
-  const int ratio = p.heads / p.kv_heads;
-  pdl_wait();
-  pdl_launch();
-  for (int i = threadIdx.x; i <= p.groups; i += kThreads) s_starts[i] = p.groups ? p.starts[i] : 0;
-  __syncthreads();
-  const int block_rows = p.team * kRows;
-  lay_out(p.groups, s_shared, s_warp, [&](int g) {
-    const int first = s_starts[g], keys = shared_keys(p, g);
-    s_source[g] = first;
-    if (first < 0 || first >= p.seqs || keys == 0) return 0;
-    const int n = min(min(max(s_starts[g + 1], first), p.seqs) - first, p.max_group);
-    int source = first;
-    while (source < first + n && length_of(p, source) < keys) ++source;
-    s_source[g] = source;
-    return source < first + n ? (keys + p.span - 1) / p.span * ((n * ratio + block_rows - 1) / block_rows) : 0;
-  });
-  lay_out(p.seqs, s_own, s_warp, [&](int seq) {
-    const int common = common_keys(p, s_starts, seq);
-    s_common[seq] = common;
-    if (blockIdx.x == 0) p.common[seq] = common;
-    return (length_of(p, seq) - common + p.span - 1) / p.span;
-  });
-  __syncthreads();
+// Where the parts are, in shared memory.
+struct Layout {
+  int* starts;                           // [groups + 1]
+  int* source;                           // [groups] first sequence that has all the shared keys
+  int* shared;                           // [groups + 1] parts of shared keys, over heads
+  int* common;                           // [sequences]
+  int* own;                              // [sequences + 1] parts of own keys
+  uint64_t* full;                        // [warps][stages] a warp's tile has arrived
+  volatile int* abort;
+  int shared_span, own_span;
+};
 
-  uint8_t* const ring = smem + warp * kRingBytes;
-  const uint32_t ring_at = smem_addr(ring), lane_at = (uint32_t)chunk_at(lane >> 4, lane & 15);
+// The parts of shared keys, or of own ones, that fall to the warp.
+template <typename T, bool kTma, bool kFew>
+__device__ __forceinline__ void run_parts(const SharedDecode& p, const Layout& at, const CUtensorMap* map_k, const CUtensorMap* map_v,
+                                          bool own, uint8_t* smem, uint32_t& used) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gq = lane >> 2, t = lane & 3;
+  const int ratio = p.heads / p.kv_heads, block_rows = p.team * kRows;
+  const int team = own ? 1 : p.team, member = warp % team, first_warp = warp - member;
+  const int teams = gridDim.x * (kWarps / team);
+  const int units = (int)min((int64_t)(own ? at.own[p.seqs] : at.shared[p.groups]) * p.kv_heads, (int64_t)1 << 30);
+  // (own keys in the other direction: who had a part more of the shared ones then has one less)
+  int unit = warp / team * gridDim.x + blockIdx.x;
+  if (own) unit = teams - 1 - unit;
+
+  auto part_of = [&](int u) {
+    Part x;
+    x.kvh = u % p.kv_heads;
+    const int v = u / p.kv_heads;
+    if (own) {
+      const int seq = last_before(at.own, p.seqs, v), chunk = v - at.own[seq], common = at.common[seq];
+      x.source = x.seq0 = seq;
+      x.row0 = 0;
+      x.rows = ratio;
+      x.t0 = (common & ~(kTile - 1)) + chunk * at.own_span;
+      x.t_lo = max(x.t0, common);
+      x.t1 = min(length_of(p, seq), x.t0 + at.own_span);
+      x.index = (common + at.shared_span - 1) / at.shared_span + chunk;
+    } else {
+      const int g = last_before(at.shared, p.groups, v), i = v - at.shared[g];
+      x.seq0 = at.starts[g];
+      x.source = at.source[g];
+      x.rows = min(min(at.starts[g + 1], p.seqs) - x.seq0, p.max_group) * ratio;
+      const int blocks = (x.rows + block_rows - 1) / block_rows;
+      x.row0 = i % blocks * block_rows;
+      x.index = i / blocks;
+      x.t0 = x.t_lo = x.index * at.shared_span;
+      x.t1 = min(shared_keys(p, g), x.t0 + at.shared_span);
+    }
+    x.tiles = (x.t1 - x.t0 + kTile - 1) / kTile;
+    return x;
+  };
+
+  // The ring: what is requested runs kStages - 1 steps (a tile of every warp of the team) ahead of what is used.  `used`
+  // counts the steps of this warp's ring, over both kinds of parts.
+  const uint32_t ring_at = smem_addr(smem + warp * kRingBytes);
+  const uint32_t full_at = smem_addr(at.full);
   const uint8_t* k_lane = (const uint8_t*)p.k_cache + (lane & 15) * 16;
   const uint8_t* v_lane = (const uint8_t*)p.v_cache + (lane & 15) * 16;
-  const float scale = p.scale * kLog2e;
-  for (int phase = 0; phase < 2; ++phase) {
-    const bool own = phase == 1;
-    const int team = own ? 1 : p.team, member = warp % team, first_warp = warp - member;
-    const int teams = gridDim.x * (kWarps / team);
-    const int units = (int)min((int64_t)(own ? s_own[p.seqs] : s_shared[p.groups]) * p.kv_heads, (int64_t)1 << 30);
-    // (the second phase in the other direction: who had a part more then has one less)
-    int unit = warp / team * gridDim.x + blockIdx.x;
-    if (own) unit = teams - 1 - unit;
-
-    auto part_of = [&](int u) {
-      Part x;
-      x.kvh = u % p.kv_heads;
-      const int v = u / p.kv_heads;
-      if (own) {
-        const int seq = last_before(s_own, p.seqs, v), chunk = v - s_own[seq], common = s_common[seq];
-        x.source = x.seq0 = seq;
-        x.row0 = 0;
-        x.rows = ratio;
-        x.t0 = common + chunk * p.span;
-        x.t1 = min(length_of(p, seq), x.t0 + p.span);
-        x.index = (common + p.span - 1) / p.span + chunk;
-      } else {
-        const int g = last_before(s_shared, p.groups, v), i = v - s_shared[g];
-        x.seq0 = s_starts[g];
-        x.source = s_source[g];
-        x.rows = min(min(s_starts[g + 1], p.seqs) - x.seq0, p.max_group) * ratio;
-        const int blocks = (x.rows + block_rows - 1) / block_rows;
-        x.row0 = i % blocks * block_rows;
-        x.index = i / blocks;
-        x.t0 = x.index * p.span;
-        x.t1 = min(shared_keys(p, g), x.t0 + p.span);
-      }
-      x.tiles = (x.t1 - x.t0 + kTile - 1) / kTile;
-      return x;
-    };
-
-    // The ring: what is requested runs kStages - 1 steps (a tile of every warp of the team) ahead of what is used.
-    int ahead_unit = unit, ahead_step = 0, stage = 0;
-    Part ahead;
-    const int* table = nullptr;
-    uint32_t row = 0;                                          // cache row and head of key 16 * tile + (lane & 15) of the next request
-    auto find_row = [&]() {
-      const int tile = ahead_step * team + member;
-      if (ahead_unit < units && tile < ahead.tiles)            // keys past the end repeat the last
-        row = cache_row(p, table, min(ahead.t0 + tile * kTile + (lane & 15), ahead.t1 - 1)) + ahead.kvh;
-    };
-    auto begin = [&]() {
-      if (ahead_unit >= units) return;
-      ahead = part_of(ahead_unit);
-      table = p.tables + (size_t)ahead.source * p.width;
-    };
-    auto request = [&](int to) {                               // and go on to the next one
-      const int tile = ahead_step * team + member;
-      if (ahead_unit < units) {
-        if (tile < ahead.tiles) {
-          const int keys = ahead.t1 - ahead.t0 - tile * kTile; // values past the end are zero, as their weights are
+  int ahead_unit = unit, ahead_step = 0;
+  uint32_t requested = used;
+  Part ahead = {};
+  const int* table = nullptr;
+  uint32_t row = 0;                      // of the next request: the tile's first cache row, or row and head of its key lane % 16
+  auto find_row = [&]() {
+    const int tile = ahead_step * team + member;
+    if (ahead_unit >= units || tile >= ahead.tiles) return;
+    if (kTma) row = cache_row(p, table, ahead.t0 + tile * kTile);
+    else row = cache_row(p, table, min(ahead.t0 + tile * kTile + (lane & 15), ahead.t1 - 1)) * p.kv_heads + ahead.kvh;  // (the last again past the end)
+  };
+  auto begin = [&]() {
+    if (ahead_unit >= units) return;
+    ahead = part_of(ahead_unit);
+    table = p.tables + (size_t)ahead.source * p.width;
+  };
+  auto request = [&]() {                 // and go on to the next one
+    const uint32_t slot = requested++ % kStages;
+    if (ahead_unit < units) {
+      const uint32_t to = ring_at + slot * kStageBytes, full = full_at + (warp * kStages + slot) * 8;
+      if (ahead_step * team + member < ahead.tiles) {
+        if (kTma) {
+          const int r = (int)__shfl_sync(0xffffffffu, row, 0), c = ahead.kvh * kDim;
+          warp_mbar_expect_tx(full, kStageBytes);
+          warp_tma_load_2d(to, map_k, c, r, full);
+          warp_tma_load_2d(to + kHalfStage / 2, map_k, c + 64, r, full);
+          warp_tma_load_2d(to + kHalfStage, map_v, c, r, full);
+          warp_tma_load_2d(to + kHalfStage * 3 / 2, map_v, c + 64, r, full);
+        } else {
 #pragma unroll
           for (int j = 0; j < kTile / 2; ++j) {                // row 2 j + lane / 16, chunk lane % 16
             const size_t from = (size_t)__shfl_sync(0xffffffffu, row, 2 * j + (lane >> 4)) * kRowBytes;
-            const uint32_t dst = ring_at + to * kStageBytes + (lane_at ^ (j & 3) << 4) + j * 2 * kRowBytes;
+            const uint32_t dst = to + chunk_at(2 * j + (lane >> 4), lane & 15);
             copy16(dst, k_lane + from, 16);
-            copy16(dst + kHalfStage, v_lane + from, 2 * j + (lane >> 4) < keys ? 16 : 0);
+            copy16(dst + kHalfStage, v_lane + from, 16);
           }
         }
-        if (++ahead_step * team >= ahead.tiles) {
-          ahead_step = 0;
-          ahead_unit += teams;
-          begin();
+      } else if (kTma && lane == 0) {
+        mbar_arrive(full);               // nothing comes
+      }
+      if (++ahead_step * team >= ahead.tiles) {
+        ahead_step = 0;
+        ahead_unit += teams;
+        begin();
+      }
+      find_row();
+    }
+    if (!kTma) cp_async_commit();
+  };
+  begin();
+  find_row();
+#pragma unroll
+  for (int s = 0; s < kStages - 1; ++s) request();
+
+  const float scale = p.scale * kLog2e;
+  constexpr int kHalves = kFew ? 1 : 2;                        // rows gq, and gq + 8
+  for (; unit < units; unit += teams) {
+    const Part part = part_of(unit);
+    const int mine = part.row0 + member * kRows;
+    uint4 q[kHalves][4];                                       // absent rows are zero
+#pragma unroll
+    for (int i = 0; i < kHalves; ++i) {
+      const int r = mine + gq + 8 * i;
+      const T* from = (const T*)p.q + (size_t)(part.seq0 + r / ratio) * p.q_stride + (size_t)(part.kvh * ratio + r % ratio) * kDim;
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        q[i][c] = r < part.rows ? *reinterpret_cast<const uint4*>(from + quarter(c, t) * 8) : make_uint4(0, 0, 0, 0);
+    }
+    float m[kHalves], l[kHalves];
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) { m[h] = -INFINITY; l[h] = 0.f; }
+    // [8 components][row gq: 2, row gq + 8: 2]; few rows: [2 of the first parts, 2 of the others]
+    float o[16][4];
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
+
+    for (int step = 0; step * team < part.tiles; ++step) {
+      const uint32_t slot = used % kStages, parity = used / kStages & 1;
+      if (!kTma) cp_async_wait<kStages - 2>();
+      if (team == 1) __syncwarp();
+      else asm volatile("bar.sync %0, %1;" ::"r"(first_warp / team + 1), "r"(team * 32) : "memory");
+      ++used;
+      request();
+      for (int w = 0; w < team; ++w) {
+        const int tile = step * team + w;
+        if (tile >= part.tiles) break;
+        const uint8_t* ks = smem + (first_warp + w) * kRingBytes + slot * kStageBytes;
+        if (kTma) mbar_wait(full_at + ((first_warp + w) * kStages + slot) * 8, parity, at.abort, p.status);
+        const int k0 = part.t0 + tile * kTile;
+        // (products on one sum are kept apart: it takes some twenty-five cycles from one to the next)
+        float s[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[i][e] = 0.f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const uint4 ka = *reinterpret_cast<const uint4*>(ks + chunk_at(gq, quarter(c, t)));
+          const uint4 kb = *reinterpret_cast<const uint4*>(ks + chunk_at(8 + gq, quarter(c, t)));
+          const uint4 q0 = q[0][c], q1 = kFew ? make_uint4(0, 0, 0, 0) : q[kHalves - 1][c];
+          const uint32_t a0[4] = {q0.x, q1.x, q0.y, q1.y}, a1[4] = {q0.z, q1.z, q0.w, q1.w};
+          mma16816<T>(s[0], a0, ka.x, ka.y);
+          mma16816<T>(s[1], a0, kb.x, kb.y);
+          mma16816<T>(s[2], a1, ka.z, ka.w);
+          mma16816<T>(s[3], a1, kb.z, kb.w);
         }
-        find_row();
-      }
-      cp_async_commit();
-    };
-    begin();
-    find_row();
+        float x[2][kHalves][2];                                // [keys k0 + 8 i][row gq + 8 h][key 2 t + e]
 #pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) request(s);
-
-    for (; unit < units; unit += teams) {
-      const Part part = part_of(unit);
-      // rows gq and gq + 8 of the warp's 16: components 32 c + 8 t ... + 7; absent rows are zero
-      const int mine = part.row0 + member * kRows;
-      uint4 q[2][4];
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = mine + gq + 8 * i;
-        const T* from = (const T*)p.q + (size_t)(part.seq0 + r / ratio) * p.q_stride + (size_t)(part.kvh * ratio + r % ratio) * kDim;
+          for (int h = 0; h < kHalves; ++h)
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-          q[i][c] = r < part.rows ? *reinterpret_cast<const uint4*>(from + c * 32 + t * 8) : make_uint4(0, 0, 0, 0);
-      }
-      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-      float o[16][4];                                          // [8 components][row gq: 2, row gq + 8: 2]
+            for (int e = 0; e < 2; ++e) x[i][h][e] = (s[i][2 * h + e] + s[2 + i][2 * h + e]) * scale;
+        // keys that do not count: no score, and a value that is zero, as their weights are
+        const bool whole = k0 >= part.t_lo && k0 + kTile <= part.t1;
+        uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
+        if (!whole) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
+          for (int i = 0; i < 2; ++i) {
+            keep[i] = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
-
-      for (int step = 0; step * team < part.tiles; ++step) {
-        cp_async_wait<kStages - 2>();
-        if (team == 1) __syncwarp();
-        else asm volatile("bar.sync %0, %1;" ::"r"(first_warp / team + 1), "r"(team * 32) : "memory");
-        request(stage == 0 ? kStages - 1 : stage - 1);
-        for (int w = 0; w < team; ++w) {
-          const int tile = step * team + w;
-          if (tile >= part.tiles) break;
-          const uint8_t* ks = smem + (first_warp + w) * kRingBytes + stage * kStageBytes;
-          const int k0 = part.t0 + tile * kTile;
-          float x[2][2][2];                                    // [keys k0 + 8 i][row gq + 8 h][key 2 t + e]
-          // (products on one sum are kept apart: it takes some thirty cycles from one to the next)
-          float s[4][4];
+            for (int e = 0; e < 2; ++e) {
+              const int key = k0 + i * 8 + 2 * t + e;
+              if (key >= part.t_lo && key < part.t1) {
+                keep[i] |= 0xffffu << 16 * e;
+              } else {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[i][e] = 0.f;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const uint4 ka = *reinterpret_cast<const uint4*>(ks + chunk_at(gq, 4 * c + t));
-            const uint4 kb = *reinterpret_cast<const uint4*>(ks + chunk_at(8 + gq, 4 * c + t));
-            const uint32_t a0[4] = {q[0][c].x, q[1][c].x, q[0][c].y, q[1][c].y};
-            const uint32_t a1[4] = {q[0][c].z, q[1][c].z, q[0][c].w, q[1][c].w};
-            mma16816<T>(s[0], a0, ka.x, ka.y);
-            mma16816<T>(s[1], a0, kb.x, kb.y);
-            mma16816<T>(s[2], a1, ka.z, ka.w);
-            mma16816<T>(s[3], a1, kb.z, kb.w);
-          }
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-              for (int e = 0; e < 2; ++e) x[i][h][e] = (s[i][2 * h + e] + s[2 + i][2 * h + e]) * scale;
-          if (k0 + kTile > part.t1) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-              for (int e = 0; e < 2; ++e)
-                if (k0 + i * 8 + 2 * t + e >= part.t1) x[i][0][e] = x[i][1][e] = -INFINITY;
-          }
-          float mx[2];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            mx[h] = fmaxf(fmaxf(x[0][h][0], x[0][h][1]), fmaxf(x[1][h][0], x[1][h][1]));
-            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-          }
-          if (__any_sync(0xffffffffu, mx[0] > m[0] + kSlack || mx[1] > m[1] + kSlack)) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float mn = fmaxf(m[h], mx[h]), c = mn == m[h] ? 1.f : exp2_of(m[h] - mn);
-              m[h] = mn;
-              l[h] *= c;
-#pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                o[j][2 * h] *= c;
-                o[j][2 * h + 1] *= c;
-              }
-            }
-          }
-          const float ms[2] = {m[0] == -INFINITY ? 0.f : m[0] - kLift<T>, m[1] == -INFINITY ? 0.f : m[1] - kLift<T>};
-          uint32_t hi[4], mid[4], low[4];
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float w0 = exp2_of(x[i][h][0] - ms[h]), w1 = exp2_of(x[i][h][1] - ms[h]);
-              l[h] += w0 + w1;
-              split_weights<T>(w0, w1, hi[2 * i + h], mid[2 * i + h], low[2 * i + h]);
-            }
-          const uint8_t* vs = ks + kHalfStage;
-#pragma unroll
-          for (int j0 = 0; j0 < 8; j0 += 4) {
-            uint32_t b[4][4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) ldsm4_t(b[j], vs + chunk_at(lane & 15, 2 * (j0 + j) + (lane >> 4)));
-#pragma unroll
-            for (int w = 0; w < 3; ++w) {
-              const uint32_t (&a)[4] = w == 0 ? hi : w == 1 ? mid : low;
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                mma16816<T>(o[2 * (j0 + j)], a, b[j][0], b[j][1]);
-                mma16816<T>(o[2 * (j0 + j) + 1], a, b[j][2], b[j][3]);
+                for (int h = 0; h < kHalves; ++h) x[i][h][e] = -INFINITY;
               }
             }
           }
         }
-        stage = stage == kStages - 1 ? 0 : stage + 1;
-      }
-      bool finite = true;
+        float mx[kHalves];
+        bool grown = false;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-        const int r = mine + gq + 8 * h, seq = part.seq0 + r / ratio;
-        if (r < part.rows && (own || s_common[seq] > 0)) {     // (otherwise it reads all of its keys by itself)
-          const size_t to = ((size_t)seq * p.heads + part.kvh * ratio + r % ratio) * p.parts + part.index;
-          float* out = p.partial + to * kDim + 2 * t;
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            finite = finite && isfinite(o[j][2 * h]) && isfinite(o[j][2 * h + 1]);
-            *reinterpret_cast<float2*>(out + j * 8) = make_float2(o[j][2 * h], o[j][2 * h + 1]);
-          }
-          if (t == 0) p.ml[to] = make_float2(m[h], l[h]);
+        for (int h = 0; h < kHalves; ++h) {
+          mx[h] = fmaxf(fmaxf(x[0][h][0], x[0][h][1]), fmaxf(x[1][h][0], x[1][h][1]));
+          mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+          mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+          grown = grown || mx[h] > m[h] + kSlack;
         }
-      }
-      if (__any_sync(0xffffffffu, !finite)) {
-        __syncwarp();
-        for (int i = 0; i < kRows; ++i) {
-          const int r = mine + i, seq = part.seq0 + r / ratio;
-          if (r >= part.rows || (!own && s_common[seq] == 0)) continue;
-          const float mr = __shfl_sync(0xffffffffu, i < 8 ? m[0] : m[1], (i & 7) * 4);
-          const size_t to = ((size_t)seq * p.heads + part.kvh * ratio + r % ratio) * p.parts + part.index;
-          const float4 v = sum_plainly<T>(p, part, r, mr);
-          *reinterpret_cast<float4*>(p.partial + to * kDim + lane * 4) = v;
+        if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+          for (int h = 0; h < kHalves; ++h) {
+            const float mn = fmaxf(m[h], mx[h]), c = mn == m[h] ? 1.f : exp2_of(m[h] - mn);
+            m[h] = mn;
+            l[h] *= c;
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+#pragma unroll
+              for (int e = kFew ? 0 : 2 * h; e < (kFew ? 4 : 2 * h + 2); ++e) o[j][e] *= c;
+          }
+        }
+        // few rows: weights of half the size, whose first parts count twice
+        uint32_t a[3][4];                                      // first, second and third parts; few rows: [second, third beside the first]
+#pragma unroll
+        for (int h = 0; h < kHalves; ++h) {
+          const float off = (m[h] == -INFINITY ? 0.f : m[h]) - (kLift<T> - kFew);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float w0 = exp2_of(x[i][h][0] - off), w1 = exp2_of(x[i][h][1] - off);
+            l[h] += w0 + w1;
+            if (kFew) {
+              uint32_t first;
+              split_weights<T>(w0, w1, 2.f, first, a[0][2 * i + 1], a[1][2 * i + 1]);
+              a[0][2 * i] = a[1][2 * i] = first;
+            } else {
+              split_weights<T>(w0, w1, 1.f, a[0][2 * i + h], a[1][2 * i + h], a[2][2 * i + h]);
+            }
+          }
+        }
+        const uint8_t* vs = ks + kHalfStage;
+#pragma unroll
+        for (int j0 = 0; j0 < 8; j0 += 4) {
+          uint32_t b[4][4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) ldsm4_t(b[j], vs + chunk_at(lane & 15, 2 * (j0 + j) + (lane >> 4)));
+          if (!whole) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) b[j][e] &= keep[e & 1];
+          }
+#pragma unroll
+          for (int w2 = 0; w2 < (kFew ? 2 : 3); ++w2)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              mma16816<T>(o[2 * (j0 + j)], a[w2], b[j][0], b[j][1]);
+              mma16816<T>(o[2 * (j0 + j) + 1], a[w2], b[j][2], b[j][3]);
+            }
         }
       }
     }
-    cp_async_wait<0>();
-    if (phase == 0) __syncthreads();                           // the rings change hands
+    bool finite = true;
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) {
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+      const int r = mine + gq + 8 * h, seq = part.seq0 + r / ratio;
+      if (r < part.rows && (own || at.common[seq] > 0)) {      // (otherwise it reads all of its keys by itself)
+        const size_t to = ((size_t)seq * p.heads + part.kvh * ratio + r % ratio) * p.parts + part.index;
+        float* out = p.partial + to * kDim + 2 * t;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          float2 v = make_float2(o[j][2 * h], o[j][2 * h + 1]);
+          if (kFew) {                                          // (an infinity is what the first parts make of it)
+            if (isfinite(v.x)) v.x += o[j][2];
+            if (isfinite(v.y)) v.y += o[j][3];
+          } else {
+            finite = finite && isfinite(v.x) && isfinite(v.y);
+          }
+          *reinterpret_cast<float2*>(out + j * 8) = v;
+        }
+        if (t == 0) p.ml[to] = make_float2(m[h], kFew ? 2.f * l[h] : l[h]);
+      }
+    }
+    if (!kFew && __any_sync(0xffffffffu, !finite)) {
+      __syncwarp();
+      for (int i = 0; i < kRows; ++i) {
+        const int r = mine + i, seq = part.seq0 + r / ratio;
+        if (r >= part.rows || (!own && at.common[seq] == 0)) continue;
+        const float mr = __shfl_sync(0xffffffffu, i < 8 ? m[0] : m[kHalves - 1], (i & 7) * 4);
+        const size_t to = ((size_t)seq * p.heads + part.kvh * ratio + r % ratio) * p.parts + part.index;
+        const float4 v = sum_plainly<T>(p, part, r, mr);
+        *reinterpret_cast<float4*>(p.partial + to * kDim + lane * 4) = v;
+      }
+    }
   }
+  if (!kTma) cp_async_wait<0>();
+  // the team's rings change hands
+  if (team == 1) __syncwarp();
+  else asm volatile("bar.sync %0, %1;" ::"r"(first_warp / team + 1), "r"(team * 32) : "memory");
+}
+
+// Keys of a part, of which `total` (over heads and blocks of rows) are dealt to `teams`: n parts for each, n being the
+// smallest number that leaves them idle for less than a tenth of the time, or the best there is.  parts(span): how many there
+// are.  Every warp tries a number; every thread of the block calls it.
+template <typename F>
+__device__ __forceinline__ int choose_span(const SharedDecode& p, int64_t total, int teams, int step, int* tried, F parts) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = warp + 1;
+  int span = 0, spent = 0;
+  for (int again = 0; again < 3; ++again) {
+    int64_t want = (total + (int64_t)teams * n - 1) / ((int64_t)teams * n);
+    if (again) want = max(want, (int64_t)span + span / 16 + 1);                // the last try took too many parts
+    span = (int)min(max((want + step - 1) / step * step, (int64_t)p.least), (int64_t)1 << 30);
+    const int64_t count = parts(span, lane);
+    spent = (int)min((count + teams - 1) / teams * span, (int64_t)1 << 30);
+    if (count <= (int64_t)teams * n || span == p.least) break;
+  }
+  if (lane == 0) { tried[2 * warp] = span; tried[2 * warp + 1] = spent; }
+  __syncthreads();
+  int best = 0;
+  for (int w = 1; w < kWarps; ++w)
+    if (tried[2 * w + 1] < tried[2 * best + 1] - tried[2 * best + 1] / 10) best = w;
+  span = tried[2 * best];
+  __syncthreads();
+  return span;
+}
+
+template <typename T, bool kTma, bool kFewShared, bool kFewOwn>
+__global__ void __launch_bounds__(kThreads, 1)
+shared_decode_kernel(const __grid_constant__ SharedDecode p, const __grid_constant__ CUtensorMap map_k,
+                     const __grid_constant__ CUtensorMap map_v) {
+  extern __shared__ uint8_t dynamic[];
+  __shared__ int s_warp[kWarps], s_tried[2 * kWarps], s_abort;
+  __shared__ int64_t s_sum[kWarps];
+  __shared__ uint64_t s_full[kWarps * kStages];
+  uint8_t* smem = dynamic + ((1024 - (smem_addr(dynamic) & 1023)) & 1023);
+  Layout at;
+  at.starts = reinterpret_cast<int*>(smem + kWarps * kRingBytes);
+  at.source = at.starts + p.groups + 1;
+  at.shared = at.source + p.groups;
+  at.common = at.shared + p.groups + 1;
+  at.own = at.common + p.seqs;
+  at.full = s_full;
+  at.abort = &s_abort;
+  if (threadIdx.x == 0) {
+    s_abort = 0;
+    if (kTma) {
+      for (int i = 0; i < kWarps * kStages; ++i) mbar_init(smem_addr(s_full + i), 1);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      fence_proxy_async();
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
+    }
+  }
+  pdl_wait();
+  pdl_launch();
+  for (int i = threadIdx.x; i <= p.groups; i += kThreads) at.starts[i] = p.groups ? p.starts[i] : 0;
+  __syncthreads();
+  const int ratio = p.heads / p.kv_heads, block_rows = p.team * kRows;
+  // sequences of a group that read together, from group g's first on, and their blocks of rows; -1: none
+  auto blocks_of = [&](int g) {
+    const int first = at.starts[g];
+    if (first < 0 || first >= p.seqs) return 0;
+    return (min(min(max(at.starts[g + 1], first), p.seqs) - first, p.max_group) * ratio + block_rows - 1) / block_rows;
+  };
+  // lengths first: what a group shares goes where its parts will be counted, a sequence's own keys likewise
+  int64_t shared_total = 0, own_total = 0;
+  for (int g = threadIdx.x; g < p.groups; g += kThreads) {
+    const int first = at.starts[g], blocks = blocks_of(g);
+    int keys = blocks > 0 ? shared_keys(p, g) : 0, source = max(first, 0);
+    if (keys > 0) {
+      const int end = first + min(min(max(at.starts[g + 1], first), p.seqs) - first, p.max_group);
+      while (source < end && length_of(p, source) < keys) ++source;
+      if (source == end) keys = 0;
+    }
+    at.source[g] = source;
+    at.shared[g] = keys;
+    shared_total += (int64_t)keys * blocks;
+  }
+  for (int seq = threadIdx.x; seq < p.seqs; seq += kThreads) {
+    const int common = common_keys(p, at.starts, seq), own = length_of(p, seq) - (common & ~(kTile - 1));
+    at.common[seq] = common;
+    at.own[seq] = length_of(p, seq) > common ? own : 0;
+    own_total += at.own[seq];
+    if (blockIdx.x == 0) p.common[seq] = common;
+  }
+  shared_total = sum_of_block(shared_total, s_sum);
+  own_total = sum_of_block(own_total, s_sum);
+  auto over = [&](int n, int lane, auto count) {
+    int64_t sum = 0;
+    for (int i = lane; i < n; i += 32) sum += count(i);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return sum * p.kv_heads;
+  };
+  at.shared_span = choose_span(p, shared_total * p.kv_heads, gridDim.x * (kWarps / p.team), p.team * kTile, s_tried, [&](int span, int lane) {
+    return over(p.groups, lane, [&](int g) { return (int64_t)((at.shared[g] + span - 1) / span) * blocks_of(g); });
+  });
+  at.own_span = choose_span(p, own_total * p.kv_heads, gridDim.x * kWarps, kTile, s_tried, [&](int span, int lane) {
+    return over(p.seqs, lane, [&](int seq) { return (int64_t)((at.own[seq] + span - 1) / span); });
+  });
+  if (blockIdx.x == 0 && threadIdx.x == 0) { p.spans[0] = at.shared_span; p.spans[1] = at.own_span; }
+  lay_out(p.groups, at.shared, s_warp, [&](int g) { return (at.shared[g] + at.shared_span - 1) / at.shared_span * blocks_of(g); });
+  lay_out(p.seqs, at.own, s_warp, [&](int seq) { return (at.own[seq] + at.own_span - 1) / at.own_span; });
+  __syncthreads();
+
+  uint32_t used = 0;
+  run_parts<T, kTma, kFewShared>(p, at, &map_k, &map_v, false, smem, used);
+  run_parts<T, kTma, kFewOwn>(p, at, &map_k, &map_v, true, smem, used);
 }
 
 // A warp per row: the parts' outputs by the weight of their maxima.
@@ -442,55 +609,77 @@ template <typename T>
 __global__ void __launch_bounds__(256) shared_join_kernel(SharedDecode p) {
   pdl_wait();
   pdl_launch();
-  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), d = (threadIdx.x & 31) * 4;
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (row >= p.seqs * p.heads) return;
-  const int seq = row / p.heads, common = p.common[seq], fresh = length_of(p, seq) - common;
-  const int parts = (common + p.span - 1) / p.span + (fresh + p.span - 1) / p.span;
+  const int seq = row / p.heads, common = p.common[seq], length = length_of(p, seq);
+  const int shared_span = p.spans[0], own_span = p.spans[1];
+  const int own = length > common ? length - (common & ~(kTile - 1)) : 0;
+  const int parts = (common + shared_span - 1) / shared_span + (own + own_span - 1) / own_span;
   const float2* ml = p.ml + (size_t)row * p.parts;
-  const float* from = p.partial + (size_t)row * p.parts * kDim + d;
+  const float* from = p.partial + (size_t)row * p.parts * kDim + lane * 4;
   float mm = -INFINITY, sum = 0.f, a[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < parts; ++i) mm = fmaxf(mm, ml[i].x);
-#pragma unroll 4
-  for (int i = 0; i < parts; ++i) {
-    const float2 w = ml[i];
-    const float4 v = *reinterpret_cast<const float4*>(from + (size_t)i * kDim);
+  for (int i = lane; i < parts; i += 32) mm = fmaxf(mm, ml[i].x);
+  mm = warp_max(mm);
+  for (int i0 = 0; i0 < parts; i0 += 32) {
+    const float2 w = i0 + lane < parts ? ml[i0 + lane] : make_float2(-INFINITY, 0.f);
     const float c = w.x == -INFINITY ? 0.f : exp2_of(w.x - mm);
     sum += w.y * c;
-    a[0] += v.x * c;
-    a[1] += v.y * c;
-    a[2] += v.z * c;
-    a[3] += v.w * c;
+    const int n = min(32, parts - i0);
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) {
+      const float4 v = *reinterpret_cast<const float4*>(from + (size_t)(i0 + i) * kDim);
+      const float ci = __shfl_sync(0xffffffffu, c, i);
+      a[0] += v.x * ci;
+      a[1] += v.y * ci;
+      a[2] += v.z * ci;
+      a[3] += v.w * ci;
+    }
   }
+  sum = warp_sum(sum);
   uint2 v = make_uint2(Cvt<T>::down(a[0] / sum, a[1] / sum), Cvt<T>::down(a[2] / sum, a[3] / sum));
   if (parts == 0) v = make_uint2(0, 0);
-  *reinterpret_cast<uint2*>((T*)p.out + (size_t)row * kDim + d) = v;
+  *reinterpret_cast<uint2*>((T*)p.out + (size_t)row * kDim + lane * 4) = v;
 }
 
 struct Plan {
-  int team, span, parts;
+  int team, least, parts;
 };
-Plan plan(int num_seqs, int num_groups, int max_group, int max_shared, int max_keys, int heads, int kv_heads) {
-  const int ratio = heads / kv_heads;
-  const int64_t shared = max_shared < max_keys ? max_shared : max_keys;
+Plan plan(int num_seqs, int max_group, int max_keys, int heads, int kv_heads) {
   Plan r;
-  const int64_t rows = (int64_t)(max_group < num_seqs ? max_group : num_seqs) * ratio;
+  const int64_t rows = (int64_t)(max_group < num_seqs ? max_group : num_seqs) * (heads / kv_heads);
   r.team = rows <= kRows ? 1 : rows <= 2 * kRows ? 2 : 4;
-  // about six parts for every team, were all lengths two thirds of the longest; no more than a row's table takes
-  const int64_t keys = (num_groups * shared * ((rows + r.team * kRows - 1) / (r.team * kRows)) * r.team + num_seqs * (max_keys - shared)) * kv_heads * 2 / 3;
-  int64_t span = keys / (148 * kWarps * 6);
-  const int64_t least = (max_keys + kMaxParts - 3) / (kMaxParts - 2);
-  if (span < least) span = least;
-  if (span < kMinSpan) span = kMinSpan;
-  r.span = (int)((span + kMinSpan - 1) / kMinSpan * kMinSpan);
-  r.parts = max_keys / r.span + 2;
+  // no part has fewer keys than this, so that a row has kMaxParts at most, whatever its lengths are
+  const int step = r.team * kTile, some = (max_keys + kMaxParts - 5) / (kMaxParts - 4), least = some > 32 ? some : 32;
+  r.least = (least + step - 1) / step * step;
+  r.parts = max_keys / r.least + 3;
   return r;
 }
 struct Scratch {
-  size_t ml, common, total;              // behind the parts' outputs
+  size_t ml, common, spans, total;       // behind the parts' outputs
 };
 Scratch scratch(int num_seqs, int heads, const Plan& r) {
   const size_t n = (size_t)num_seqs * heads * r.parts;
-  return {n * kDim * 4, n * (kDim * 4 + 8), n * (kDim * 4 + 8) + (size_t)num_seqs * 4};
+  const size_t common = n * (kDim * 4 + 8), spans = common + (size_t)num_seqs * 4;
+  return {n * kDim * 4, common, spans, spans + 8};
+}
+
+template <typename T, bool kTma, bool kFewShared, bool kFewOwn>
+int launch_form(const SharedDecode& p, const CUtensorMap& map_k, const CUtensorMap& map_v, size_t smem, cudaStream_t st) {
+  const auto kernel = shared_decode_kernel<T, kTma, kFewShared, kFewOwn>;
+  DZ_CUDA_OK(allow_smem(kernel, smem));
+  DZ_CUDA_OK(launch_ex(kernel, dim3(148), dim3(kThreads), smem, 1, st, p, map_k, map_v));
+  return DZ_OK;
+}
+template <typename T>
+int launch_decode(const SharedDecode& p, const CUtensorMap& map_k, const CUtensorMap& map_v, bool tma, bool few_shared, bool few_own,
+                  size_t smem, cudaStream_t st) {
+  if (tma)
+    return few_shared ? launch_form<T, true, true, true>(p, map_k, map_v, smem, st)
+           : few_own  ? launch_form<T, true, false, true>(p, map_k, map_v, smem, st)
+                      : launch_form<T, true, false, false>(p, map_k, map_v, smem, st);
+  return few_shared ? launch_form<T, false, true, true>(p, map_k, map_v, smem, st)
+         : few_own  ? launch_form<T, false, false, true>(p, map_k, map_v, smem, st)
+                    : launch_form<T, false, false, false>(p, map_k, map_v, smem, st);
 }
 
 }  // namespace
@@ -507,7 +696,7 @@ size_t dz_shared_attention_workspace_bytes(int num_seqs, int num_groups, int max
   if (num_seqs <= 0 || num_groups < 0 || max_group < 0 || max_shared < 0 || max_keys <= 0 || q_heads <= 0 || kv_heads <= 0 ||
       q_heads % kv_heads)
     return 0;
-  return scratch(num_seqs, q_heads, plan(num_seqs, num_groups, max_group, max_shared, max_keys, q_heads, kv_heads)).total;
+  return scratch(num_seqs, q_heads, plan(num_seqs, max_group, max_keys, q_heads, kv_heads)).total;
 }
 
 int dz_shared_attention_decode(const dz_shared_attention_args* a, void* stream) {
@@ -527,7 +716,7 @@ int dz_shared_attention_decode(const dz_shared_attention_args* a, void* stream) 
   const int64_t keys = (int64_t)a->table_width * a->block_size;
   if (a->cache_rows * a->kv_heads > 0x7fffffff || a->block_size > (1 << 30)) return DZ_ERR_TOO_LARGE;
   if (a->num_seqs > kMaxSeqs || a->num_groups > kMaxSeqs || keys > (1 << 30) || a->kv_heads > 4096) return DZ_ERR_TOO_LARGE;
-  const Plan r = plan(a->num_seqs, a->num_groups, a->max_group, a->max_shared, (int)keys, a->q_heads, a->kv_heads);
+  const Plan r = plan(a->num_seqs, a->max_group, (int)keys, a->q_heads, a->kv_heads);
   // parts are counted in 32 bits
   if ((int64_t)a->num_seqs * 2 * r.parts * a->kv_heads > (1 << 30)) return DZ_ERR_TOO_LARGE;
   if (!a->workspace || a->workspace_bytes < dz_shared_attention_workspace_bytes(a->num_seqs, a->num_groups, a->max_group, a->max_shared,
@@ -543,14 +732,26 @@ int dz_shared_attention_decode(const dz_shared_attention_args* a, void* stream) 
   const SharedDecode p = {a->qkv, a->q_row_stride, a->out, a->k_cache, a->v_cache, (uint32_t)(a->cache_rows - 1),
                           (uint32_t)((a->cache_rows - 1) / a->block_size), a->block_tables, a->table_width,
                           a->block_size, magic, 31 + log, a->seq_lens, a->group_starts, a->shared_lens, a->num_groups, a->num_seqs, a->q_heads,
-                          a->kv_heads, a->scale, a->max_group, a->max_shared, r.team, r.span, r.parts,
-                          reinterpret_cast<float*>(ws), reinterpret_cast<float2*>(ws + at.ml), reinterpret_cast<int*>(ws + at.common)};
+                          a->kv_heads, a->scale, a->max_group, a->max_shared, r.team, r.least, r.parts,
+                          reinterpret_cast<float*>(ws), reinterpret_cast<float2*>(ws + at.ml), reinterpret_cast<int*>(ws + at.common), reinterpret_cast<int*>(ws + at.spans), a->status};
   cudaStream_t st = (cudaStream_t)stream;
   const int rows = a->num_seqs * a->q_heads;
-  const size_t smem = (size_t)kWarps * kRingBytes + (size_t)(3 * a->num_groups + 2 * a->num_seqs + 3) * 4;
-  DZ_DISPATCH16(a->dtype, DZ_CUDA_OK(allow_smem(shared_decode_kernel<T>, smem));
-                DZ_CUDA_OK(launch_ex(shared_decode_kernel<T>, dim3(148), dim3(kThreads), smem, 1, st, p));
-                DZ_CUDA_OK(launch_pdl(shared_join_kernel<T>, dim3((rows + 7) / 8), dim3(256), st, p)));
+  const size_t smem = 1024 + (size_t)kWarps * kRingBytes + (size_t)(3 * a->num_groups + 2 * a->num_seqs + 3) * 4;
+  // a tile of keys is in one page, and TMA's coordinates and strides reach
+  const bool tma = a->block_size % kTile == 0 && a->cache_rows >= kTile;
+  CUtensorMap map_k = {}, map_v = {};
+  if (tma) {
+    const int dt = a->dtype == DZ_DTYPE_BF16;
+    int rc = encode_map(&map_k, a->k_cache, (int)a->cache_rows, a->kv_heads * kDim, kTile, dt);
+    if (rc == DZ_OK) rc = encode_map(&map_v, a->v_cache, (int)a->cache_rows, a->kv_heads * kDim, kTile, dt);
+    if (rc != DZ_OK) return rc;
+  }
+  const int ratio = a->q_heads / a->kv_heads;
+  const bool few_own = ratio <= kEight, few_shared = few_own && r.team == 1 && (int64_t)a->max_group * ratio <= kEight;
+  int rc = DZ_OK;
+  DZ_DISPATCH16(a->dtype, rc = launch_decode<T>(p, map_k, map_v, tma, few_shared, few_own, smem, st);
+                if (rc == DZ_OK) DZ_CUDA_OK(launch_pdl(shared_join_kernel<T>, dim3((rows + 7) / 8), dim3(256), st, p)));
+  if (rc != DZ_OK) return rc;
   return DZ_OK;
 }
 

@@ -186,8 +186,8 @@ def _workspace(device, nbytes: int) -> torch.Tensor:
 
 
 def read_status(device=None) -> int:
-    """Reads and clears the status words the SBMM, window attention, latent attention, expert and chunkwise recurrence
-    kernels leave in the current stream's workspaces (0 = ok, DZ_ERR_TIMEOUT = a bounded device-side wait ran
+    """Reads and clears the status words the SBMM, window attention, latent attention, shared attention, expert and chunkwise
+    recurrence kernels leave in the current stream's workspaces (0 = ok, DZ_ERR_TIMEOUT = a bounded device-side wait ran
     out, DZ_ERR_INVALID_ARG = a wrong `tokens_sorted` promise).  Synchronises."""
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     found = 0
@@ -1141,7 +1141,7 @@ def shared_attention_decode(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: t
         qkv.data_ptr(), qkv.stride(0) if b > 1 else width, out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0],
         block_tables.data_ptr(), block_tables.shape[1], block_size, seq_lens.data_ptr(), group_starts.data_ptr(),
         shared_lens.data_ptr(), groups, b, max_group, max_shared, q_heads, kv_heads, 128, float(scale), ws.data_ptr(), size,
-        _dtype_code(qkv))
+        _dtype_code(qkv), _zeroed_scratch("status", qkv.device, 256).data_ptr())
     check(lib().dz_shared_attention_decode(ctypes.byref(args), _stream()), "dz_shared_attention_decode")
     return out
 

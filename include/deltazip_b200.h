@@ -600,6 +600,7 @@ typedef struct dz_shared_attention_args {
   void* workspace;
   size_t workspace_bytes;
   int32_t dtype;
+  int32_t* status;          /* device word for a wait that ran out, may be NULL */
 } dz_shared_attention_args;
 size_t dz_shared_attention_workspace_bytes(int num_seqs, int num_groups, int max_group, int max_shared, int max_keys, int q_heads,
                                            int kv_heads);
