@@ -21,11 +21,11 @@
 // Rows are those of 16 x 8 x 16 warp MMAs.
 //   scores   S[rows, 8 keys] += Q K^T; the order of the 128 products of a score is free, so a lane's 16-byte piece of
 //            a key row serves two MMAs as it lies.
-//   output   O[rows, 128] += P V: a 32-bit weight is the sum of three 16-bit parts, all of its bits.  V comes
-//            transposed by ldmatrix.
-// With up to eight rows the other eight of an MMA carry the second and third parts: two MMAs of half the first part each,
-// one with the second and one with the third beside it, 48 MMAs a tile instead of 64; and an infinity in V is found in the
-// first part's sums.  With more rows, where a part of a weight that is zero makes a NaN of an infinity, output that is
+//   output   O[rows, 128] += P V: a weight is the sum of two (fp16) or three (bf16) 16-bit parts.  V comes transposed by
+//            ldmatrix.
+// With up to eight rows the other eight of an MMA carry the other parts (fp16: one MMA with the first and the second part;
+// bf16: two of half the first part each, one with the second and one with the third beside it); and an infinity in V is
+// found in the first part's sums.  With more rows, where a part of a weight that is zero makes a NaN of an infinity, output that is
 // not finite is summed again in plain 32-bit arithmetic, which few ever need.
 // A row's weights are taken relative to a maximum that moves only when it has grown by kSlack: moving it costs a
 // multiplication of the whole output, and among 16 rows one has a new maximum in nearly every tile.
@@ -39,7 +39,7 @@ constexpr int kDim = 128, kRows = 16;                          // rows of a warp
 constexpr int kWarps = 12, kThreads = kWarps * 32, kStages = 2, kTile = 16;    // keys per tile
 constexpr int kRowBytes = kDim * 2, kHalfStage = kTile * kRowBytes, kStageBytes = 2 * kHalfStage;
 constexpr int kRingBytes = kStages * kStageBytes;
-constexpr int kMaxSeqs = 1536;           // also groups: what the layout of the parts takes of shared memory
+constexpr int kMaxSeqs = 1024;           // also groups: what the layout of the parts takes of shared memory
 constexpr int kMaxParts = 64;            // of a row
 constexpr int kEight = 8;                // rows that leave half of an MMA's to the weights' parts
 
@@ -75,17 +75,23 @@ __device__ __forceinline__ int chunk_at(int r, int c) { return (c >> 3) * (kHalf
 // The chunk of K and Q that a lane (t = lane % 4) has of the c-th quarter.
 __device__ __forceinline__ int quarter(int c, int t) { return (c >> 1) * 8 + 2 * t + (c & 1); }
 
-// Scores are kept times log2 e, and weights are 2^(score - maximum + kLift), at most 2^(kLift + kSlack).  Two of them as three
-// 16-bit numbers each: all bits (fp16: of weights above 2^-12 of the largest; below, what is lost is at most 2^-36 of it,
-// which no sum with the largest can hold).
+// Scores are kept times log2 e, and weights are 2^(score - maximum + kLift), at most 2^(kLift + kSlack).  They enter the
+// products with V as sums of 16-bit numbers: two of fp16 hold 22 bits, as many as the exponential's own error leaves (of weights
+// above 2^-12 of the largest; below, what is lost is at most 2^-35 of it, which no sum with the largest can hold), bf16
+// takes three for its 24.
 constexpr int kSlack = 4;
 template <typename T> constexpr int kLift = 0;
 template <> constexpr int kLift<__half> = 11;
+template <typename T> constexpr int kParts = 3;
+template <> constexpr int kParts<__half> = 2;
 template <typename T>
 __device__ __forceinline__ void split_weights(float a, float b, float times, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
   hi = Cvt<T>::down(a, b);
   const float2 h = Cvt<T>::up(hi);
-  split_pair<T>(times * (a - h.x), times * (b - h.y), mid, lo);    // of what the first part leaves, `times` over
+  a = times * (a - h.x);                 // of what the first part leaves, `times` over
+  b = times * (b - h.y);
+  if constexpr (kParts<T> == 3) split_pair<T>(a, b, mid, lo);
+  else mid = Cvt<T>::down(a, b);
 }
 
 __device__ __forceinline__ float exp2_of(float x) {            // (what is below 2^-126 is zero)
@@ -94,10 +100,6 @@ __device__ __forceinline__ float exp2_of(float x) {            // (what is below
   return y;
 }
 
-// How many keys a group shares, as far as they are read together.
-__device__ __forceinline__ int shared_keys(const SharedDecode& p, int g) {
-  return min(max(p.shared[g], 0), min(p.max_shared, p.width * p.block_size));
-}
 __device__ __forceinline__ int length_of(const SharedDecode& p, int seq) { return min(max(p.lens[seq], 0), p.width * p.block_size); }
 
 // The last of `n` entries that starts at or before x.
@@ -109,29 +111,15 @@ __device__ __forceinline__ int last_before(const int* starts, int n, int x) {
   }
   return lo;
 }
-// The shared keys that sequence `seq` reads with its group (0: none, it reads all of its keys by itself).
-__device__ __forceinline__ int common_keys(const SharedDecode& p, const int* starts, int seq) {
-  if (p.groups == 0) return 0;
-  const int g = last_before(starts, p.groups, seq), first = starts[g];
-  if (first < 0 || seq < first || seq >= starts[g + 1] || seq - first >= p.max_group) return 0;
-  const int n = shared_keys(p, g);
-  return length_of(p, seq) >= n ? n : 0;
-}
 
+// A word, or zero.  (Loaded four at a time, words lie together in registers, and every MMA moves those it takes from two rows.)
+__device__ __forceinline__ uint32_t word(const void* p, bool there) {
+  uint32_t v;
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\tmov.u32 %0, 0;\n\t@p ld.global.b32 %0, [%1];\n\t}" : "=r"(v) : "l"(p), "r"((int)there));
+  return v;
+}
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {      // the rest of 16 becomes zero
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-
-__device__ __forceinline__ int64_t sum_of_block(int64_t x, int64_t* part) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = x;
-  __syncthreads();
-  x = 0;
-  for (int w = 0; w < kWarps; ++w) x += part[w];
-  __syncthreads();
-  return x;
 }
 
 // Running sums of count(i), i < n, in front of each i and at sums[n]; count may read sums[i].  Every thread of the block
@@ -204,9 +192,11 @@ __device__ __noinline__ float4 sum_plainly(const SharedDecode& p, Part part, int
 struct Layout {
   int* starts;                           // [groups + 1]
   int* source;                           // [groups] first sequence that has all the shared keys
-  int* shared;                           // [groups + 1] parts of shared keys, over heads
-  int* common;                           // [sequences]
-  int* own;                              // [sequences + 1] parts of own keys
+  int* keys;                             // [groups] shared keys
+  int* shared;                           // [groups + 1] parts of shared keys in front of each group's, over heads
+  int* length;                           // [sequences]
+  int* common;                           // [sequences] keys that a sequence reads with its group
+  int* own;                              // [sequences + 1] parts of own keys, likewise
   uint64_t* full;                        // [warps][stages] a warp's tile has arrived
   volatile int* abort;
   int shared_span, own_span;
@@ -236,7 +226,7 @@ __device__ __forceinline__ void run_parts(const SharedDecode& p, const Layout& a
       x.rows = ratio;
       x.t0 = (common & ~(kTile - 1)) + chunk * at.own_span;
       x.t_lo = max(x.t0, common);
-      x.t1 = min(length_of(p, seq), x.t0 + at.own_span);
+      x.t1 = min(at.length[seq], x.t0 + at.own_span);
       x.index = (common + at.shared_span - 1) / at.shared_span + chunk;
     } else {
       const int g = last_before(at.shared, p.groups, v), i = v - at.shared[g];
@@ -247,7 +237,7 @@ __device__ __forceinline__ void run_parts(const SharedDecode& p, const Layout& a
       x.row0 = i % blocks * block_rows;
       x.index = i / blocks;
       x.t0 = x.t_lo = x.index * at.shared_span;
-      x.t1 = min(shared_keys(p, g), x.t0 + at.shared_span);
+      x.t1 = min(at.keys[g], x.t0 + at.shared_span);
     }
     x.tiles = (x.t1 - x.t0 + kTile - 1) / kTile;
     return x;
@@ -315,6 +305,7 @@ __device__ __forceinline__ void run_parts(const SharedDecode& p, const Layout& a
 
   const float scale = p.scale * kLog2e;
   constexpr int kHalves = kFew ? 1 : 2;                        // rows gq, and gq + 8
+  constexpr bool kDoubled = kFew && kParts<T> == 3;            // weights of half the size, whose first parts count twice
   for (; unit < units; unit += teams) {
     const Part part = part_of(unit);
     const int mine = part.row0 + member * kRows;
@@ -324,8 +315,11 @@ __device__ __forceinline__ void run_parts(const SharedDecode& p, const Layout& a
       const int r = mine + gq + 8 * i;
       const T* from = (const T*)p.q + (size_t)(part.seq0 + r / ratio) * p.q_stride + (size_t)(part.kvh * ratio + r % ratio) * kDim;
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-        q[i][c] = r < part.rows ? *reinterpret_cast<const uint4*>(from + quarter(c, t) * 8) : make_uint4(0, 0, 0, 0);
+      for (int c = 0; c < 4; ++c) {
+        const T* piece = from + quarter(c, t) * 8;
+        q[i][c] = make_uint4(word(piece, r < part.rows), word(piece + 2, r < part.rows), word(piece + 4, r < part.rows),
+                             word(piece + 6, r < part.rows));
+      }
     }
     float m[kHalves], l[kHalves];
 #pragma unroll
@@ -414,19 +408,17 @@ __device__ __forceinline__ void run_parts(const SharedDecode& p, const Layout& a
               for (int e = kFew ? 0 : 2 * h; e < (kFew ? 4 : 2 * h + 2); ++e) o[j][e] *= c;
           }
         }
-        // few rows: weights of half the size, whose first parts count twice
-        uint32_t a[3][4];                                      // first, second and third parts; few rows: [second, third beside the first]
+        uint32_t a[3][4];                                      // first, second and third parts; few rows: the first with each of the others
 #pragma unroll
         for (int h = 0; h < kHalves; ++h) {
-          const float off = (m[h] == -INFINITY ? 0.f : m[h]) - (kLift<T> - kFew);
+          const float off = (m[h] == -INFINITY ? 0.f : m[h]) - (kLift<T> - kDoubled);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const float w0 = exp2_of(x[i][h][0] - off), w1 = exp2_of(x[i][h][1] - off);
             l[h] += w0 + w1;
-            if (kFew) {
-              uint32_t first;
-              split_weights<T>(w0, w1, 2.f, first, a[0][2 * i + 1], a[1][2 * i + 1]);
-              a[0][2 * i] = a[1][2 * i] = first;
+            if constexpr (kFew) {
+              split_weights<T>(w0, w1, kDoubled ? 2.f : 1.f, a[0][2 * i], a[0][2 * i + 1], a[1][2 * i + 1]);
+              a[1][2 * i] = a[0][2 * i];
             } else {
               split_weights<T>(w0, w1, 1.f, a[0][2 * i + h], a[1][2 * i + h], a[2][2 * i + h]);
             }
@@ -445,7 +437,7 @@ __device__ __forceinline__ void run_parts(const SharedDecode& p, const Layout& a
               for (int e = 0; e < 4; ++e) b[j][e] &= keep[e & 1];
           }
 #pragma unroll
-          for (int w2 = 0; w2 < (kFew ? 2 : 3); ++w2)
+          for (int w2 = 0; w2 < kParts<T> - kFew; ++w2)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               mma16816<T>(o[2 * (j0 + j)], a[w2], b[j][0], b[j][1]);
@@ -474,7 +466,7 @@ __device__ __forceinline__ void run_parts(const SharedDecode& p, const Layout& a
           }
           *reinterpret_cast<float2*>(out + j * 8) = v;
         }
-        if (t == 0) p.ml[to] = make_float2(m[h], kFew ? 2.f * l[h] : l[h]);
+        if (t == 0) p.ml[to] = make_float2(m[h], kDoubled ? 2.f * l[h] : l[h]);
       }
     }
     if (!kFew && __any_sync(0xffffffffu, !finite)) {
@@ -497,27 +489,27 @@ __device__ __forceinline__ void run_parts(const SharedDecode& p, const Layout& a
 
 // Keys of a part, of which `total` (over heads and blocks of rows) are dealt to `teams`: n parts for each, n being the
 // smallest number that leaves them idle for less than a tenth of the time, or the best there is.  parts(span): how many there
-// are.  Every warp tries a number; every thread of the block calls it.
+// are.  Warp `n` - 1 of those that look for it tries n.
+constexpr int kTries = kWarps / 2;
 template <typename F>
-__device__ __forceinline__ int choose_span(const SharedDecode& p, int64_t total, int teams, int step, int* tried, F parts) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = warp + 1;
-  int span = 0, spent = 0;
+__device__ __forceinline__ void try_span(const SharedDecode& p, float total, int teams, int n, int step, float* tried, F parts) {
+  int span = 0, count = 0;
   for (int again = 0; again < 3; ++again) {
-    int64_t want = (total + (int64_t)teams * n - 1) / ((int64_t)teams * n);
-    if (again) want = max(want, (int64_t)span + span / 16 + 1);                // the last try took too many parts
-    span = (int)min(max((want + step - 1) / step * step, (int64_t)p.least), (int64_t)1 << 30);
-    const int64_t count = parts(span, lane);
-    spent = (int)min((count + teams - 1) / teams * span, (int64_t)1 << 30);
-    if (count <= (int64_t)teams * n || span == p.least) break;
+    const float want = again ? span * 1.0625f + 1.f : total / (float)(teams * n);     // (the last try took too many parts)
+    span = max((int)(fminf(want, 1e9f) / (float)step + 0.999f) * step, p.least);
+    count = parts(span);
+    if (count <= teams * n || span == p.least) break;
   }
-  if (lane == 0) { tried[2 * warp] = span; tried[2 * warp + 1] = spent; }
-  __syncthreads();
+  if ((threadIdx.x & 31) == 0) {
+    tried[2 * n - 2] = (float)span;
+    tried[2 * n - 1] = ceilf((float)count / (float)teams) * (float)span;
+  }
+}
+__device__ __forceinline__ int best_span(const float* tried) {
   int best = 0;
-  for (int w = 1; w < kWarps; ++w)
-    if (tried[2 * w + 1] < tried[2 * best + 1] - tried[2 * best + 1] / 10) best = w;
-  span = tried[2 * best];
-  __syncthreads();
-  return span;
+  for (int i = 1; i < kTries; ++i)
+    if (tried[2 * i + 1] < 0.9f * tried[2 * best + 1]) best = i;
+  return (int)tried[2 * best];
 }
 
 template <typename T, bool kTma, bool kFewShared, bool kFewOwn>
@@ -525,15 +517,17 @@ __global__ void __launch_bounds__(kThreads, 1)
 shared_decode_kernel(const __grid_constant__ SharedDecode p, const __grid_constant__ CUtensorMap map_k,
                      const __grid_constant__ CUtensorMap map_v) {
   extern __shared__ uint8_t dynamic[];
-  __shared__ int s_warp[kWarps], s_tried[2 * kWarps], s_abort;
-  __shared__ int64_t s_sum[kWarps];
+  __shared__ int s_warp[kWarps], s_abort;
+  __shared__ float s_total[2][kWarps], s_tried[2][2 * kTries];
   __shared__ uint64_t s_full[kWarps * kStages];
   uint8_t* smem = dynamic + ((1024 - (smem_addr(dynamic) & 1023)) & 1023);
   Layout at;
   at.starts = reinterpret_cast<int*>(smem + kWarps * kRingBytes);
   at.source = at.starts + p.groups + 1;
-  at.shared = at.source + p.groups;
-  at.common = at.shared + p.groups + 1;
+  at.keys = at.source + p.groups;
+  at.shared = at.keys + p.groups;
+  at.length = at.shared + p.groups + 1;
+  at.common = at.length + p.seqs;
   at.own = at.common + p.seqs;
   at.full = s_full;
   at.abort = &s_abort;
@@ -549,51 +543,64 @@ shared_decode_kernel(const __grid_constant__ SharedDecode p, const __grid_consta
   }
   pdl_wait();
   pdl_launch();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, most = p.width * p.block_size;
   for (int i = threadIdx.x; i <= p.groups; i += kThreads) at.starts[i] = p.groups ? p.starts[i] : 0;
+  for (int i = threadIdx.x; i < p.groups; i += kThreads) at.keys[i] = min(max(p.shared[i], 0), min(p.max_shared, most));
+  for (int i = threadIdx.x; i < p.seqs; i += kThreads) at.length[i] = min(max(p.lens[i], 0), most);
   __syncthreads();
   const int ratio = p.heads / p.kv_heads, block_rows = p.team * kRows;
-  // sequences of a group that read together, from group g's first on, and their blocks of rows; -1: none
-  auto blocks_of = [&](int g) {
+  // the sequences of group g that read together, and the blocks of rows they make
+  auto members = [&](int g) {
     const int first = at.starts[g];
-    if (first < 0 || first >= p.seqs) return 0;
-    return (min(min(max(at.starts[g + 1], first), p.seqs) - first, p.max_group) * ratio + block_rows - 1) / block_rows;
+    return first < 0 || first >= p.seqs ? 0 : min(min(max(at.starts[g + 1], first), p.seqs) - first, p.max_group);
   };
-  // lengths first: what a group shares goes where its parts will be counted, a sequence's own keys likewise
-  int64_t shared_total = 0, own_total = 0;
-  for (int g = threadIdx.x; g < p.groups; g += kThreads) {
-    const int first = at.starts[g], blocks = blocks_of(g);
-    int keys = blocks > 0 ? shared_keys(p, g) : 0, source = max(first, 0);
-    if (keys > 0) {
-      const int end = first + min(min(max(at.starts[g + 1], first), p.seqs) - first, p.max_group);
-      while (source < end && length_of(p, source) < keys) ++source;
-      if (source == end) keys = 0;
-    }
-    at.source[g] = source;
-    at.shared[g] = keys;
-    shared_total += (int64_t)keys * blocks;
-  }
+  auto blocks_of = [&](int g) { return (members(g) * ratio + block_rows - 1) / block_rows; };
+  float shared_total = 0.f, own_total = 0.f;
   for (int seq = threadIdx.x; seq < p.seqs; seq += kThreads) {
-    const int common = common_keys(p, at.starts, seq), own = length_of(p, seq) - (common & ~(kTile - 1));
+    int common = 0;                      // a sequence that is shorter than its group's shared keys reads all of its own by itself
+    if (p.groups > 0) {
+      const int g = last_before(at.starts, p.groups, seq), first = at.starts[g];
+      if (first >= 0 && seq >= first && seq < at.starts[g + 1] && seq - first < p.max_group && at.length[seq] >= at.keys[g])
+        common = at.keys[g];
+    }
+    const int own = at.length[seq] > common ? at.length[seq] - (common & ~(kTile - 1)) : 0;
     at.common[seq] = common;
-    at.own[seq] = length_of(p, seq) > common ? own : 0;
-    own_total += at.own[seq];
+    at.own[seq] = own;
+    own_total += (float)own;
     if (blockIdx.x == 0) p.common[seq] = common;
   }
-  shared_total = sum_of_block(shared_total, s_sum);
-  own_total = sum_of_block(own_total, s_sum);
-  auto over = [&](int n, int lane, auto count) {
-    int64_t sum = 0;
-    for (int i = lane; i < n; i += 32) sum += count(i);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    return sum * p.kv_heads;
-  };
-  at.shared_span = choose_span(p, shared_total * p.kv_heads, gridDim.x * (kWarps / p.team), p.team * kTile, s_tried, [&](int span, int lane) {
-    return over(p.groups, lane, [&](int g) { return (int64_t)((at.shared[g] + span - 1) / span) * blocks_of(g); });
-  });
-  at.own_span = choose_span(p, own_total * p.kv_heads, gridDim.x * kWarps, kTile, s_tried, [&](int span, int lane) {
-    return over(p.seqs, lane, [&](int seq) { return (int64_t)((at.own[seq] + span - 1) / span); });
-  });
+  for (int g = threadIdx.x; g < p.groups; g += kThreads) {
+    const int n = members(g), first = at.starts[g];
+    int source = first;
+    while (source < first + n && at.length[source] < at.keys[g]) ++source;
+    at.source[g] = source;
+    at.shared[g] = source < first + n ? at.keys[g] : 0;
+    shared_total += (float)at.shared[g] * (float)blocks_of(g);
+  }
+  shared_total = warp_sum(shared_total);
+  own_total = warp_sum(own_total);
+  if (lane == 0) { s_total[0][warp] = shared_total; s_total[1][warp] = own_total; }
+  __syncthreads();
+  {
+    const int kind = warp / kTries, n = warp % kTries + 1;
+    const float total = warp_sum(lane < kWarps ? s_total[kind][lane] : 0.f) * (float)p.kv_heads;
+    auto over = [&](int many, auto count) {                    // (numbers beyond any launch's are cut off)
+      float sum = 0.f;
+      for (int i = lane; i < many; i += 32) sum += (float)count(i);
+      return (int)fminf(warp_sum(sum) * (float)p.kv_heads, 1e9f);
+    };
+    if (kind == 0)
+      try_span(p, total, gridDim.x * (kWarps / p.team), n, p.team * kTile, s_tried[0], [&](int span) {
+        return over(p.groups, [&](int g) { return (at.shared[g] + span - 1) / span * blocks_of(g); });
+      });
+    else
+      try_span(p, total, gridDim.x * kWarps, n, kTile, s_tried[1], [&](int span) {
+        return over(p.seqs, [&](int seq) { return (at.own[seq] + span - 1) / span; });
+      });
+  }
+  __syncthreads();
+  at.shared_span = best_span(s_tried[0]);
+  at.own_span = best_span(s_tried[1]);
   if (blockIdx.x == 0 && threadIdx.x == 0) { p.spans[0] = at.shared_span; p.spans[1] = at.own_span; }
   lay_out(p.groups, at.shared, s_warp, [&](int g) { return (at.shared[g] + at.shared_span - 1) / at.shared_span * blocks_of(g); });
   lay_out(p.seqs, at.own, s_warp, [&](int seq) { return (at.own[seq] + at.own_span - 1) / at.own_span; });
@@ -736,7 +743,7 @@ int dz_shared_attention_decode(const dz_shared_attention_args* a, void* stream) 
                           reinterpret_cast<float*>(ws), reinterpret_cast<float2*>(ws + at.ml), reinterpret_cast<int*>(ws + at.common), reinterpret_cast<int*>(ws + at.spans), a->status};
   cudaStream_t st = (cudaStream_t)stream;
   const int rows = a->num_seqs * a->q_heads;
-  const size_t smem = 1024 + (size_t)kWarps * kRingBytes + (size_t)(3 * a->num_groups + 2 * a->num_seqs + 3) * 4;
+  const size_t smem = 1024 + (size_t)kWarps * kRingBytes + (size_t)(4 * a->num_groups + 3 * a->num_seqs + 3) * 4;
   // a tile of keys is in one page, and TMA's coordinates and strides reach
   const bool tma = a->block_size % kTile == 0 && a->cache_rows >= kTile;
   CUtensorMap map_k = {}, map_v = {};
