@@ -10,15 +10,21 @@
 // them; nothing is counted or waited for between CTAs.
 //
 // One CTA of twelve warps per SM stays for the whole launch.  It first lays out all parts (how long they are and how many,
-// by scans over groups and sequences in shared memory, the same in every CTA), then its warps take every n-th part: of shared
-// keys in teams of one, two or four warps with 16 rows each over the same key tiles, then of own keys each by itself.  A
-// warp's ring of key tiles runs on from part to part, so that the end of one is not waited for.  Neighbouring parts have
+// by scans over groups and sequences in shared memory, the same in every CTA), then takes every n-th part: of shared keys as
+// a whole on tcgen05 where a group has more than 16 rows, otherwise warp by warp; then of own keys warp by warp.  A warp's
+// ring of key tiles runs on from part to part, so that the end of one is not waited for.  Neighbouring parts have
 // neighbouring heads of the same cache rows, and go to different SMs.
 //
 // Tiles are 16 keys that begin at a multiple of 16.  Where pages are whole tiles, a tile is four TMA boxes of 16 rows x 128
 // bytes; otherwise each row is copied by itself.
 //
-// Rows are those of 16 x 8 x 16 warp MMAs.
+// On tcgen05 up to 128 rows are the lanes of tensor memory, tiles are 64 keys: S = Q K^T in two buffers, a thread per row takes
+// its scores and puts the weights' parts in their place, O += P V with the parts one after the other.  Four warps do that,
+// two bring K and V (five stages), one issues the MMAs: the next tile's scores are computed under this one's softmax.  (On
+// warp MMAs, 64 rows took two and a half times the time of the cache's bytes.)
+//
+// Warp by warp, rows are those of 16 x 8 x 16 MMAs (teams of two or four warps share key tiles, 16 rows each, where pages
+// are not whole tiles).
 //   scores   S[rows, 8 keys] += Q K^T; the order of the 128 products of a score is free, so a lane's 16-byte piece of
 //            a key row serves two MMAs as it lies.
 //   output   O[rows, 128] += P V: a weight is the sum of two (fp16) or three (bf16) 16-bit parts.  V comes transposed by
@@ -29,6 +35,8 @@
 // not finite is summed again in plain 32-bit arithmetic, which few ever need.
 // A row's weights are taken relative to a maximum that moves only when it has grown by kSlack: moving it costs a
 // multiplication of the whole output, and among 16 rows one has a new maximum in nearly every tile.
+#include <type_traits>
+
 #include "dz_elem.cuh"
 #include "dz_tc.cuh"
 
@@ -202,6 +210,22 @@ struct Layout {
   int shared_span, own_span;
 };
 
+__device__ __forceinline__ Part shared_part(const SharedDecode& p, const Layout& at, int u, int block_rows) {
+  Part x;
+  x.kvh = u % p.kv_heads;
+  const int v = u / p.kv_heads, g = last_before(at.shared, p.groups, v), i = v - at.shared[g];
+  x.seq0 = at.starts[g];
+  x.source = at.source[g];
+  x.rows = min(min(at.starts[g + 1], p.seqs) - x.seq0, p.max_group) * (p.heads / p.kv_heads);
+  const int blocks = (x.rows + block_rows - 1) / block_rows;
+  x.row0 = i % blocks * block_rows;
+  x.index = i / blocks;
+  x.t0 = x.t_lo = x.index * at.shared_span;
+  x.t1 = min(at.keys[g], x.t0 + at.shared_span);
+  x.tiles = (x.t1 - x.t0 + kTile - 1) / kTile;
+  return x;
+}
+
 // The parts of shared keys, or of own ones, that fall to the warp.
 template <typename T, bool kTma, bool kFew>
 __device__ __forceinline__ void run_parts(const SharedDecode& p, const Layout& at, const CUtensorMap* map_k, const CUtensorMap* map_v,
@@ -216,29 +240,17 @@ __device__ __forceinline__ void run_parts(const SharedDecode& p, const Layout& a
   if (own) unit = teams - 1 - unit;
 
   auto part_of = [&](int u) {
+    if (!own) return shared_part(p, at, u, block_rows);
     Part x;
     x.kvh = u % p.kv_heads;
-    const int v = u / p.kv_heads;
-    if (own) {
-      const int seq = last_before(at.own, p.seqs, v), chunk = v - at.own[seq], common = at.common[seq];
-      x.source = x.seq0 = seq;
-      x.row0 = 0;
-      x.rows = ratio;
-      x.t0 = (common & ~(kTile - 1)) + chunk * at.own_span;
-      x.t_lo = max(x.t0, common);
-      x.t1 = min(at.length[seq], x.t0 + at.own_span);
-      x.index = (common + at.shared_span - 1) / at.shared_span + chunk;
-    } else {
-      const int g = last_before(at.shared, p.groups, v), i = v - at.shared[g];
-      x.seq0 = at.starts[g];
-      x.source = at.source[g];
-      x.rows = min(min(at.starts[g + 1], p.seqs) - x.seq0, p.max_group) * ratio;
-      const int blocks = (x.rows + block_rows - 1) / block_rows;
-      x.row0 = i % blocks * block_rows;
-      x.index = i / blocks;
-      x.t0 = x.t_lo = x.index * at.shared_span;
-      x.t1 = min(at.keys[g], x.t0 + at.shared_span);
-    }
+    const int v = u / p.kv_heads, seq = last_before(at.own, p.seqs, v), chunk = v - at.own[seq], common = at.common[seq];
+    x.source = x.seq0 = seq;
+    x.row0 = 0;
+    x.rows = ratio;
+    x.t0 = (common & ~(kTile - 1)) + chunk * at.own_span;
+    x.t_lo = max(x.t0, common);
+    x.t1 = min(at.length[seq], x.t0 + at.own_span);
+    x.index = (common + at.shared_span - 1) / at.shared_span + chunk;
     x.tiles = (x.t1 - x.t0 + kTile - 1) / kTile;
     return x;
   };
@@ -487,18 +499,242 @@ __device__ __forceinline__ void run_parts(const SharedDecode& p, const Layout& a
   else asm volatile("bar.sync %0, %1;" ::"r"(first_warp / team + 1), "r"(team * 32) : "memory");
 }
 
+// The parts of shared keys that fall to the CTA, on tcgen05.
+constexpr int kTcRows = 128, kTcKeys = 64, kTcStages = 5;
+constexpr int kTcSlabQ = kTcRows * 128, kTcSlab = kTcKeys * 128, kTcQ = 2 * kTcSlabQ, kTcStage = 4 * kTcSlab;
+constexpr int kTcBuffer = 96, kTcOut = 2 * kTcBuffer;          // columns of tensor memory: scores and weights' parts, twice; outputs
+static_assert(kTcQ + kTcStages * kTcStage <= kWarps * kRingBytes, "the rings' place holds it");
+struct TcBarriers {
+  uint64_t full[kTcStages], empty[kTcStages], scores[2], weights[2], products, queries, outputs;
+};
+
+template <typename T>
+__device__ __forceinline__ void run_rows_tc(const SharedDecode& p, const Layout& at, const CUtensorMap* map_k, const CUtensorMap* map_v,
+                                            uint8_t* smem, TcBarriers& bar, uint32_t tmem) {
+  constexpr int DT = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, ratio = p.heads / p.kv_heads;
+  const int units = (int)min((int64_t)at.shared[p.groups] * p.kv_heads, (int64_t)1 << 30);
+  const uint32_t s_q = smem_addr(smem), s_kv = s_q + kTcQ;
+  auto wait = [&](uint64_t& b, uint32_t parity) { mbar_wait(smem_addr(&b), parity, at.abort, p.status); };
+  auto tiles_of = [](const Part& x) { return (x.t1 - x.t0 + kTcKeys - 1) / kTcKeys; };
+  uint32_t c = 0, n = 0;                                       // tiles and parts so far
+  if (warp == 4 || warp == 5) {
+    // ---- copies: K by one warp, V by the other ----
+    const bool values = warp == 5;
+    for (int u = blockIdx.x; u < units; u += gridDim.x) {
+      const Part part = shared_part(p, at, u, kTcRows);
+      const int* table = p.tables + (size_t)part.source * p.width;
+      for (int j = 0, tiles = tiles_of(part); j < tiles; ++j, ++c) {
+        const int key0 = part.t0 + j * kTcKeys, valid = min(kTcKeys, part.t1 - key0), boxes = (valid + kTile - 1) / kTile;
+        const uint32_t st = c % kTcStages, dst = s_kv + st * kTcStage + (values ? 2 * kTcSlab : 0), full = smem_addr(&bar.full[st]);
+        const uint32_t row = lane < boxes ? cache_row(p, table, key0 + lane * kTile) : 0;
+        wait(bar.empty[st], ((c / kTcStages) & 1) ^ 1);
+        __syncwarp();
+        if (values && valid < kTcKeys) {                       // rows past the end have no weight, and must not be NaN
+          for (int i = boxes * kTile * 8 + lane; i < kTcKeys * 8; i += 32)
+            for (int s = 0; s < 2; ++s) sts128(dst + s * kTcSlab + i * 16, make_uint4(0, 0, 0, 0));
+          fence_proxy_async();
+          __syncwarp();
+        }
+        const bool cut = values && valid % kTile != 0;         // so are those of the last box, once it is here
+        if (!cut) {
+          warp_mbar_expect_tx(full, boxes * kTile * 128 * 2);
+          for (int b = 0; b < boxes; ++b) {
+            const int r = (int)__shfl_sync(0xffffffffu, row, b);
+            for (int s = 0; s < 2; ++s)
+              warp_tma_load_2d(dst + s * kTcSlab + b * kTile * 128, values ? map_v : map_k, part.kvh * kDim + s * 64, r, full);
+          }
+        } else {
+          warp_mbar_expect_tx(full, (boxes - 1) * kTile * 128 * 2);
+          for (int b = 0; b + 1 < boxes; ++b) {
+            const int r = (int)__shfl_sync(0xffffffffu, row, b);
+            for (int s = 0; s < 2; ++s)
+              warp_tma_load_2d(dst + s * kTcSlab + b * kTile * 128, map_v, part.kvh * kDim + s * 64, r, full);
+          }
+          // the last box row by row: 16 chunks of each, those that count
+          const uint32_t r0 = __shfl_sync(0xffffffffu, row, boxes - 1);
+          for (int i = lane; i < kTile * 16; i += 32) {
+            const int r = i >> 4, chunk = i & 15, at_row = (boxes - 1) * kTile + r;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (at_row < valid)
+              v = *reinterpret_cast<const uint4*>((const T*)p.v_cache + ((size_t)min(r0 + r, p.last_row) * p.kv_heads + part.kvh) * kDim + chunk * 8);
+            sts128(dst + (chunk >> 3) * kTcSlab + at_row * 128 + (((chunk ^ at_row) & 7) << 4), v);
+          }
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(full);
+        }
+        if (!cut && values && lane == 0) mbar_arrive(full);    // (three arrivals: K, V, and V's last box)
+      }
+    }
+  } else if (warp == 6) {
+    // ---- MMA issue ----
+    const uint32_t id_s = make_idesc<DT>(kTcKeys, false), id_o = make_idesc<DT>(kDim, false) | (1u << 16);       // V transposed
+    auto scores = [&](uint32_t c) {
+      const uint32_t st = c % kTcStages;
+      wait(bar.full[st], (c / kTcStages) & 1);
+      __syncwarp();
+      tc_fence_after();
+      const uint32_t a = desc_lo(s_q), b = desc_lo(s_kv + st * kTcStage), d = tmem + (c & 1) * kTcBuffer;
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) warp_umma_ss(d, a + s * (kTcSlabQ >> 4) + 2 * k, b + s * (kTcSlab >> 4) + 2 * k, id_s, s + k > 0);
+      warp_umma_commit(smem_addr(&bar.scores[c & 1]));
+    };
+    for (int u = blockIdx.x; u < units; u += gridDim.x, ++n) {
+      const int tiles = tiles_of(shared_part(p, at, u, kTcRows));
+      wait(bar.queries, n & 1);
+      __syncwarp();
+      scores(c);
+      if (tiles > 1) scores(c + 1);
+      for (int j = 0; j < tiles; ++j, ++c) {
+        const uint32_t st = c % kTcStages, buffer = tmem + (c & 1) * kTcBuffer;
+        wait(bar.weights[c & 1], (c >> 1) & 1);
+        __syncwarp();
+        tc_fence_after();
+        const uint32_t v = desc_lo_mn(s_kv + st * kTcStage + 2 * kTcSlab, kTcSlab);
+#pragma unroll
+        for (int k = 0; k < kTcKeys / 16; ++k)                 // 16 keys: 2048 bytes of V, 8 columns of a part
+#pragma unroll
+          for (int w = 0; w < kParts<T>; ++w)
+            warp_umma_ts(tmem + kTcOut, buffer + w * 32 + k * 8, v + k * 128, id_o, j > 0 || k > 0 || w > 0);
+        warp_umma_commit(smem_addr(&bar.empty[st]));
+        warp_umma_commit(smem_addr(&bar.products));
+        if (j + 2 < tiles) scores(c + 2);                      // behind the product that reads these columns' weights
+        if (j + 1 == tiles) warp_umma_commit(smem_addr(&bar.outputs));
+      }
+    }
+  } else if (warp < 4) {
+    // ---- softmax: a thread per row ----
+    const float scale = p.scale * kLog2e;
+    const int r = threadIdx.x;
+    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+    for (int u = blockIdx.x; u < units; u += gridDim.x, ++n) {
+      const Part part = shared_part(p, at, u, kTcRows);
+      const int row = part.row0 + r, tiles = tiles_of(part), seq = part.seq0 + row / ratio;
+      const bool there = row < part.rows, any = part.row0 + warp * 32 < part.rows;       // the row; any of the warp's
+      {
+        const T* from = (const T*)p.q + (size_t)seq * p.q_stride + (size_t)(part.kvh * ratio + row % ratio) * kDim;
+#pragma unroll 4
+        for (int i = 0; i < 16; ++i) {
+          const uint4 v = there ? *reinterpret_cast<const uint4*>(from + i * 8) : make_uint4(0, 0, 0, 0);
+          sts128(s_q + (i >> 3) * kTcSlabQ + r * 128 + (((i ^ r) & 7) << 4), v);
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_addr(&bar.queries));
+      }
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < tiles; ++j, ++c) {
+        const uint32_t t_s = tmem + (c & 1) * kTcBuffer + lanes;
+        wait(bar.scores[c & 1], (c >> 1) & 1);
+        __syncwarp();
+        tc_fence_after();
+        if (any) {
+          float s[kTcKeys];
+          tmem_ld32(t_s, s);
+          tmem_ld32(t_s + 32, s + 32);
+          tmem_wait_ld();
+          // (a negative scale turns the order round: the maximum is taken of what is scaled)
+#pragma unroll
+          for (int i = 0; i < kTcKeys; ++i) s[i] *= scale;
+          const int valid = part.t1 - part.t0 - j * kTcKeys;
+          if (valid < kTcKeys) {
+#pragma unroll
+            for (int i = 0; i < kTcKeys; ++i) s[i] = i < valid ? s[i] : -INFINITY;
+          }
+          float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+          for (int i = 4; i < kTcKeys; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          float f = 1.f;
+          if (top > m + kSlack) {
+            f = exp2_of(m - top);
+            m = top;
+            l *= f;
+          }
+          const float off = (m == -INFINITY ? 0.f : m) - kLift<T>;
+          float sum[2] = {0.f, 0.f};
+#pragma unroll
+          for (int i = 0; i < kTcKeys; i += 32) {
+            uint32_t parts[3][16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float a = exp2_of(s[i + 2 * e] - off), b = exp2_of(s[i + 2 * e + 1] - off);
+              sum[0] += a;
+              sum[1] += b;
+              split_weights<T>(a, b, 1.f, parts[0][e], parts[1][e], parts[2][e]);
+            }
+#pragma unroll
+            for (int w = 0; w < kParts<T>; ++w) tmem_st16(t_s + w * 32 + i / 2, parts[w]);
+          }
+          l += sum[0] + sum[1];
+          if (j > 0 && __any_sync(0xffffffffu, f != 1.f)) {
+            wait(bar.products, (c - 1) & 1);                   // O holds the products so far
+            __syncwarp();
+            tc_fence_after();
+            for (int i = 0; i < kDim; i += 32) {
+              float o[32];
+              tmem_ld32(tmem + kTcOut + lanes + i, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] *= f;
+              tmem_st16(tmem + kTcOut + lanes + i, reinterpret_cast<const uint32_t*>(o));
+              tmem_st16(tmem + kTcOut + lanes + i + 16, reinterpret_cast<const uint32_t*>(o + 16));
+            }
+          }
+          tmem_wait_st();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_addr(&bar.weights[c & 1]));
+      }
+      wait(bar.outputs, n & 1);
+      __syncwarp();
+      tc_fence_after();
+      if (!any) continue;
+      const bool mine = there && at.common[min(seq, p.seqs - 1)] > 0;      // (otherwise it reads all of its keys by itself)
+      const size_t to = ((size_t)seq * p.heads + part.kvh * ratio + row % ratio) * p.parts + part.index;
+      bool finite = true;
+      for (int i = 0; i < kDim; i += 32) {
+        float o[32];
+        tmem_ld32(tmem + kTcOut + lanes + i, o);
+        tmem_wait_ld();
+        if (mine) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            finite = finite && isfinite(o[e]) && isfinite(o[e + 1]) && isfinite(o[e + 2]) && isfinite(o[e + 3]);
+            *reinterpret_cast<float4*>(p.partial + to * kDim + i + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          }
+        }
+      }
+      if (mine) p.ml[to] = make_float2(m, l);
+      uint32_t again = __ballot_sync(0xffffffffu, !finite);
+      __syncwarp();
+      for (; again; again &= again - 1) {
+        const int from = __ffs(again) - 1;
+        const float4 v = sum_plainly<T>(p, part, __shfl_sync(0xffffffffu, row, from), __shfl_sync(0xffffffffu, m, from));
+        const unsigned long long place = __shfl_sync(0xffffffffu, (unsigned long long)to, from);
+        *reinterpret_cast<float4*>(p.partial + place * kDim + lane * 4) = v;
+      }
+    }
+  }
+}
+
 // Keys of a part, of which `total` (over heads and blocks of rows) are dealt to `teams`: n parts for each, n being the
 // smallest number that leaves them idle for less than a tenth of the time, or the best there is.  parts(span): how many there
 // are.  Warp `n` - 1 of those that look for it tries n.
 constexpr int kTries = kWarps / 2;
 template <typename F>
 __device__ __forceinline__ void try_span(const SharedDecode& p, float total, int teams, int n, int step, float* tried, F parts) {
+  const int least = (p.least + step - 1) / step * step;
   int span = 0, count = 0;
   for (int again = 0; again < 3; ++again) {
     const float want = again ? span * 1.0625f + 1.f : total / (float)(teams * n);     // (the last try took too many parts)
-    span = max((int)(fminf(want, 1e9f) / (float)step + 0.999f) * step, p.least);
+    span = max((int)(fminf(want, 1e9f) / (float)step + 0.999f) * step, least);
     count = parts(span);
-    if (count <= teams * n || span == p.least) break;
+    if (count <= teams * n || span == least) break;
   }
   if ((threadIdx.x & 31) == 0) {
     tried[2 * n - 2] = (float)span;
@@ -512,7 +748,8 @@ __device__ __forceinline__ int best_span(const float* tried) {
   return (int)tried[2 * best];
 }
 
-template <typename T, bool kTma, bool kFewShared, bool kFewOwn>
+enum { kByTeams, kFewRows, kOnTc };      // how shared keys are taken
+template <typename T, bool kTma, int kShared, bool kFewOwn>
 __global__ void __launch_bounds__(kThreads, 1)
 shared_decode_kernel(const __grid_constant__ SharedDecode p, const __grid_constant__ CUtensorMap map_k,
                      const __grid_constant__ CUtensorMap map_v) {
@@ -520,6 +757,8 @@ shared_decode_kernel(const __grid_constant__ SharedDecode p, const __grid_consta
   __shared__ int s_warp[kWarps], s_abort;
   __shared__ float s_total[2][kWarps], s_tried[2][2 * kTries];
   __shared__ uint64_t s_full[kWarps * kStages];
+  __shared__ TcBarriers s_tc;
+  __shared__ uint32_t s_tmem;
   uint8_t* smem = dynamic + ((1024 - (smem_addr(dynamic) & 1023)) & 1023);
   Layout at;
   at.starts = reinterpret_cast<int*>(smem + kWarps * kRingBytes);
@@ -535,6 +774,19 @@ shared_decode_kernel(const __grid_constant__ SharedDecode p, const __grid_consta
     s_abort = 0;
     if (kTma) {
       for (int i = 0; i < kWarps * kStages; ++i) mbar_init(smem_addr(s_full + i), 1);
+      if (kShared == kOnTc) {
+        for (int i = 0; i < kTcStages; ++i) {
+          mbar_init(smem_addr(&s_tc.full[i]), 3);
+          mbar_init(smem_addr(&s_tc.empty[i]), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+          mbar_init(smem_addr(&s_tc.scores[i]), 1);
+          mbar_init(smem_addr(&s_tc.weights[i]), 4);
+        }
+        mbar_init(smem_addr(&s_tc.products), 1);
+        mbar_init(smem_addr(&s_tc.queries), 4);
+        mbar_init(smem_addr(&s_tc.outputs), 1);
+      }
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
       fence_proxy_async();
       asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
@@ -548,7 +800,8 @@ shared_decode_kernel(const __grid_constant__ SharedDecode p, const __grid_consta
   for (int i = threadIdx.x; i < p.groups; i += kThreads) at.keys[i] = min(max(p.shared[i], 0), min(p.max_shared, most));
   for (int i = threadIdx.x; i < p.seqs; i += kThreads) at.length[i] = min(max(p.lens[i], 0), most);
   __syncthreads();
-  const int ratio = p.heads / p.kv_heads, block_rows = p.team * kRows;
+  const int ratio = p.heads / p.kv_heads, block_rows = kShared == kOnTc ? kTcRows : p.team * kRows;
+  const int shared_teams = kShared == kOnTc ? gridDim.x : gridDim.x * (kWarps / p.team);
   // the sequences of group g that read together, and the blocks of rows they make
   auto members = [&](int g) {
     const int first = at.starts[g];
@@ -590,7 +843,7 @@ shared_decode_kernel(const __grid_constant__ SharedDecode p, const __grid_consta
       return (int)fminf(warp_sum(sum) * (float)p.kv_heads, 1e9f);
     };
     if (kind == 0)
-      try_span(p, total, gridDim.x * (kWarps / p.team), n, p.team * kTile, s_tried[0], [&](int span) {
+      try_span(p, total, shared_teams, n, kShared == kOnTc ? kTcKeys : p.team * kTile, s_tried[0], [&](int span) {
         return over(p.groups, [&](int g) { return (at.shared[g] + span - 1) / span * blocks_of(g); });
       });
     else
@@ -607,7 +860,32 @@ shared_decode_kernel(const __grid_constant__ SharedDecode p, const __grid_consta
   __syncthreads();
 
   uint32_t used = 0;
-  run_parts<T, kTma, kFewShared>(p, at, &map_k, &map_v, false, smem, used);
+  if constexpr (kShared == kOnTc) {
+    if ((int64_t)at.shared[p.groups] * p.kv_heads > (int64_t)blockIdx.x) {       // the CTA has a part of shared keys
+      if (warp == 6) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s_tmem)), "n"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+      }
+      tc_fence_before();
+      __syncthreads();
+      tc_fence_after();
+      const uint32_t tmem = s_tmem;
+      run_rows_tc<T>(p, at, &map_k, &map_v, smem, s_tc, tmem);
+      tc_fence_before();
+      __syncthreads();
+      if (s_abort) {                                           // let copies and MMAs under way end
+        const unsigned long long t0 = globaltimer();
+        while (globaltimer() - t0 < 200000ull) __nanosleep(1000);
+        __syncthreads();
+      }
+      if (warp == 6) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
+      }
+    }
+  } else {
+    run_parts<T, kTma, kShared == kFewRows>(p, at, &map_k, &map_v, false, smem, used);
+  }
   run_parts<T, kTma, kFewOwn>(p, at, &map_k, &map_v, true, smem, used);
 }
 
@@ -655,7 +933,8 @@ Plan plan(int num_seqs, int max_group, int max_keys, int heads, int kv_heads) {
   Plan r;
   const int64_t rows = (int64_t)(max_group < num_seqs ? max_group : num_seqs) * (heads / kv_heads);
   r.team = rows <= kRows ? 1 : rows <= 2 * kRows ? 2 : 4;
-  // no part has fewer keys than this, so that a row has kMaxParts at most, whatever its lengths are
+  // no part has fewer keys than this (64 of shared keys on tcgen05: it is rounded up there), so that a row has kMaxParts at
+  // most, whatever its lengths are
   const int step = r.team * kTile, some = (max_keys + kMaxParts - 5) / (kMaxParts - 4), least = some > 32 ? some : 32;
   r.least = (least + step - 1) / step * step;
   r.parts = max_keys / r.least + 3;
@@ -670,23 +949,26 @@ Scratch scratch(int num_seqs, int heads, const Plan& r) {
   return {n * kDim * 4, common, spans, spans + 8};
 }
 
-template <typename T, bool kTma, bool kFewShared, bool kFewOwn>
+template <typename T, bool kTma, int kShared, bool kFewOwn>
 int launch_form(const SharedDecode& p, const CUtensorMap& map_k, const CUtensorMap& map_v, size_t smem, cudaStream_t st) {
-  const auto kernel = shared_decode_kernel<T, kTma, kFewShared, kFewOwn>;
+  const auto kernel = shared_decode_kernel<T, kTma, kShared, kFewOwn>;
   DZ_CUDA_OK(allow_smem(kernel, smem));
   DZ_CUDA_OK(launch_ex(kernel, dim3(148), dim3(kThreads), smem, 1, st, p, map_k, map_v));
   return DZ_OK;
 }
 template <typename T>
-int launch_decode(const SharedDecode& p, const CUtensorMap& map_k, const CUtensorMap& map_v, bool tma, bool few_shared, bool few_own,
-                  size_t smem, cudaStream_t st) {
+int launch_decode(const SharedDecode& p, const CUtensorMap& map_k, const CUtensorMap& map_v, bool tma, size_t smem, cudaStream_t st) {
+  const int ratio = p.heads / p.kv_heads;
+  const bool few_own = ratio <= kEight, few_shared = few_own && (int64_t)p.max_group * ratio <= kEight;
+  if (tma && p.team > 1)
+    return few_own ? launch_form<T, true, kOnTc, true>(p, map_k, map_v, smem, st) : launch_form<T, true, kOnTc, false>(p, map_k, map_v, smem, st);
   if (tma)
-    return few_shared ? launch_form<T, true, true, true>(p, map_k, map_v, smem, st)
-           : few_own  ? launch_form<T, true, false, true>(p, map_k, map_v, smem, st)
-                      : launch_form<T, true, false, false>(p, map_k, map_v, smem, st);
-  return few_shared ? launch_form<T, false, true, true>(p, map_k, map_v, smem, st)
-         : few_own  ? launch_form<T, false, false, true>(p, map_k, map_v, smem, st)
-                    : launch_form<T, false, false, false>(p, map_k, map_v, smem, st);
+    return few_shared ? launch_form<T, true, kFewRows, true>(p, map_k, map_v, smem, st)
+           : few_own  ? launch_form<T, true, kByTeams, true>(p, map_k, map_v, smem, st)
+                      : launch_form<T, true, kByTeams, false>(p, map_k, map_v, smem, st);
+  return few_shared ? launch_form<T, false, kFewRows, true>(p, map_k, map_v, smem, st)
+         : few_own  ? launch_form<T, false, kByTeams, true>(p, map_k, map_v, smem, st)
+                    : launch_form<T, false, kByTeams, false>(p, map_k, map_v, smem, st);
 }
 
 }  // namespace
@@ -753,10 +1035,8 @@ int dz_shared_attention_decode(const dz_shared_attention_args* a, void* stream) 
     if (rc == DZ_OK) rc = encode_map(&map_v, a->v_cache, (int)a->cache_rows, a->kv_heads * kDim, kTile, dt);
     if (rc != DZ_OK) return rc;
   }
-  const int ratio = a->q_heads / a->kv_heads;
-  const bool few_own = ratio <= kEight, few_shared = few_own && r.team == 1 && (int64_t)a->max_group * ratio <= kEight;
   int rc = DZ_OK;
-  DZ_DISPATCH16(a->dtype, rc = launch_decode<T>(p, map_k, map_v, tma, few_shared, few_own, smem, st);
+  DZ_DISPATCH16(a->dtype, rc = launch_decode<T>(p, map_k, map_v, tma, smem, st);
                 if (rc == DZ_OK) DZ_CUDA_OK(launch_pdl(shared_join_kernel<T>, dim3((rows + 7) / 8), dim3(256), st, p)));
   if (rc != DZ_OK) return rc;
   return DZ_OK;

@@ -299,6 +299,17 @@ __device__ __forceinline__ void warp_umma_ss(uint32_t d, uint32_t a_lo, uint32_t
       "r"(a_lo), "r"(b_lo), "r"(kDescHi), "r"(idesc), "r"(acc)
       : "memory");
 }
+// As warp_umma_ss, with the first operand in tensor memory.
+__device__ __forceinline__ void warp_umma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 db;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 db, {%2, %3};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(kDescHi), "r"(idesc), "r"(acc)
+      : "memory");
+}
 // One 2:4-sparse MMA (32 dense k): compressed A and metadata in tensor memory, B in shared memory.
 __device__ __forceinline__ void warp_umma_ts_sp(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t e_tmem, uint32_t idesc,
                                                 uint32_t acc) {

@@ -74,18 +74,6 @@ __device__ __forceinline__ void cp_async16_u32(uint32_t dst, const void* src, bo
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
 }
 
-// As warp_umma_ss, with the first operand in tensor memory.
-__device__ __forceinline__ void warp_umma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p, e;\n\t.reg .b64 db;\n\t"
-      "elect.sync _|e, 0xffffffff;\n\t"
-      "setp.ne.b32 p, %5, 0;\n\t"
-      "mov.b64 db, {%2, %3};\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}" ::"r"(d),
-      "r"(a), "r"(b_lo), "r"(kDescHi), "r"(idesc), "r"(acc)
-      : "memory");
-}
-
 template <typename T, int kStages>
 __global__ void __launch_bounds__(kThreadsTc, 1)
 window_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kv,
