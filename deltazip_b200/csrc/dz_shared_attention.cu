@@ -19,9 +19,10 @@
 // bytes; otherwise each row is copied by itself.
 //
 // On tcgen05 up to 128 rows are the lanes of tensor memory, tiles are 64 keys: S = Q K^T in two buffers, a thread per row takes
-// its scores and puts the weights' parts in their place, O += P V with the parts one after the other.  Four warps do that,
-// two bring K and V (five stages), one issues the MMAs: the next tile's scores are computed under this one's softmax.  (On
-// warp MMAs, 64 rows took two and a half times the time of the cache's bytes.)
+// its scores and puts the weights' parts in their place, O += P V with the parts one after the other.  Four warps do that for
+// the even tiles and four for the odd ones, each with a maximum, a sum and an output of its own, which are joined at the
+// part's end; two warps bring K and V (five stages), one issues the MMAs.  (On warp MMAs, 64 rows took two and a half times
+// the time of the cache's bytes, with four warps on all tiles 1.6 times: the softmax is what takes longest.)
 //
 // Warp by warp, rows are those of 16 x 8 x 16 MMAs (teams of two or four warps share key tiles, 16 rows each, where pages
 // are not whole tiles).
@@ -474,7 +475,7 @@ __device__ __forceinline__ void run_parts(const SharedDecode& p, const Layout& a
             if (isfinite(v.x)) v.x += o[j][2];
             if (isfinite(v.y)) v.y += o[j][3];
           } else {
-            finite = finite && isfinite(v.x) && isfinite(v.y);
+            finite = finite && ((isfinite(v.x) && isfinite(v.y)) || !(l[h] == l[h]));       // (a sum that is NaN stays one)
           }
           *reinterpret_cast<float2*>(out + j * 8) = v;
         }
@@ -502,11 +503,47 @@ __device__ __forceinline__ void run_parts(const SharedDecode& p, const Layout& a
 // The parts of shared keys that fall to the CTA, on tcgen05.
 constexpr int kTcRows = 128, kTcKeys = 64, kTcStages = 5;
 constexpr int kTcSlabQ = kTcRows * 128, kTcSlab = kTcKeys * 128, kTcQ = 2 * kTcSlabQ, kTcStage = 4 * kTcSlab;
-constexpr int kTcBuffer = 96, kTcOut = 2 * kTcBuffer;          // columns of tensor memory: scores and weights' parts, twice; outputs
+constexpr int kTcBuffer = 96, kTcOut = 2 * kTcBuffer;          // columns of tensor memory: scores and weights' parts, twice; two outputs
 static_assert(kTcQ + kTcStages * kTcStage <= kWarps * kRingBytes, "the rings' place holds it");
 struct TcBarriers {
-  uint64_t full[kTcStages], empty[kTcStages], scores[2], weights[2], products, queries, outputs;
+  uint64_t full[kTcStages], empty[kTcStages], scores[2], weights[2], products[2], queries, outputs, odd;
+  float m[kTcRows], l[kTcRows];                                // of the odd tiles
 };
+
+// Pairs of 32-bit operations in one instruction.
+__device__ __forceinline__ unsigned long long pair_of(float a, float b) {
+  unsigned long long v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ void halves_of(unsigned long long v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ unsigned long long fma_pair(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ unsigned long long add_pair(unsigned long long a, unsigned long long b) {
+  unsigned long long d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// Two weights in their parts.  bf16: the first part is the upper half of the float as it stands, the second that of what it
+// leaves (which is exact), the third the rest, rounded.
+template <typename T>
+__device__ __forceinline__ void cut_weights(float a, float b, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    auto cut = [](float& a, float& b, uint32_t& part) {
+      const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+      part = __byte_perm(ua, ub, 0x7632);
+      halves_of(fma_pair(pair_of(__uint_as_float(ua & 0xffff0000u), __uint_as_float(ub & 0xffff0000u)), pair_of(-1.f, -1.f), pair_of(a, b)), a, b);
+    };
+    cut(a, b, hi);
+    cut(a, b, mid);
+    lo = Cvt<T>::down(a, b);
+  } else {
+    split_weights<T>(a, b, 1.f, hi, mid, lo);
+  }
+}
 
 template <typename T>
 __device__ __forceinline__ void run_rows_tc(const SharedDecode& p, const Layout& at, const CUtensorMap* map_k, const CUtensorMap* map_v,
@@ -598,37 +635,44 @@ __device__ __forceinline__ void run_rows_tc(const SharedDecode& p, const Layout&
         for (int k = 0; k < kTcKeys / 16; ++k)                 // 16 keys: 2048 bytes of V, 8 columns of a part
 #pragma unroll
           for (int w = 0; w < kParts<T>; ++w)
-            warp_umma_ts(tmem + kTcOut, buffer + w * 32 + k * 8, v + k * 128, id_o, j > 0 || k > 0 || w > 0);
+            warp_umma_ts(tmem + kTcOut + (j & 1) * kDim, buffer + w * 32 + k * 8, v + k * 128, id_o, j > 1 || k > 0 || w > 0);
         warp_umma_commit(smem_addr(&bar.empty[st]));
-        warp_umma_commit(smem_addr(&bar.products));
+        warp_umma_commit(smem_addr(&bar.products[j & 1]));
         if (j + 2 < tiles) scores(c + 2);                      // behind the product that reads these columns' weights
         if (j + 1 == tiles) warp_umma_commit(smem_addr(&bar.outputs));
       }
     }
-  } else if (warp < 4) {
-    // ---- softmax: a thread per row ----
-    const float scale = p.scale * kLog2e;
-    const int r = threadIdx.x;
-    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+  } else if (warp < 4 || warp >= 8) {
+    // ---- softmax: a thread per row, of every other tile ----
+    const int odd = warp >> 3, w4 = warp & 3, r = w4 * 32 + lane;
+    // scores rise with q.k: a negative scale is a turned query's, a scale of zero that of a query of zero
+    const float scale = p.scale == 0.f ? 1.f : fabsf(p.scale) * kLog2e;
+    const uint32_t lanes = (uint32_t)(w4 * 32) << 16, t_o = tmem + kTcOut + odd * kDim + lanes;
+    uint32_t k = 0;                                            // tiles of this kind so far
     for (int u = blockIdx.x; u < units; u += gridDim.x, ++n) {
       const Part part = shared_part(p, at, u, kTcRows);
       const int row = part.row0 + r, tiles = tiles_of(part), seq = part.seq0 + row / ratio;
-      const bool there = row < part.rows, any = part.row0 + warp * 32 < part.rows;       // the row; any of the warp's
-      {
+      const bool there = row < part.rows, any = part.row0 + w4 * 32 < part.rows;         // the row; any of the warp's
+      if (!odd) {
         const T* from = (const T*)p.q + (size_t)seq * p.q_stride + (size_t)(part.kvh * ratio + row % ratio) * kDim;
+        const uint32_t turn = p.scale < 0.f ? 0x80008000u : 0u;
 #pragma unroll 4
         for (int i = 0; i < 16; ++i) {
-          const uint4 v = there ? *reinterpret_cast<const uint4*>(from + i * 8) : make_uint4(0, 0, 0, 0);
+          uint4 v = there && p.scale != 0.f ? *reinterpret_cast<const uint4*>(from + i * 8) : make_uint4(0, 0, 0, 0);
+          v = make_uint4(v.x ^ turn, v.y ^ turn, v.z ^ turn, v.w ^ turn);
           sts128(s_q + (i >> 3) * kTcSlabQ + r * 128 + (((i ^ r) & 7) << 4), v);
         }
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_addr(&bar.queries));
+      } else {
+        wait(bar.queries, n & 1);                              // the even tiles' warps are through with the part before
+        __syncwarp();
       }
       float m = -INFINITY, l = 0.f;
-      for (int j = 0; j < tiles; ++j, ++c) {
-        const uint32_t t_s = tmem + (c & 1) * kTcBuffer + lanes;
-        wait(bar.scores[c & 1], (c >> 1) & 1);
+      for (int j = odd; j < tiles; j += 2) {
+        const uint32_t tile = c + j, t_s = tmem + (tile & 1) * kTcBuffer + lanes;
+        wait(bar.scores[tile & 1], (tile >> 1) & 1);
         __syncwarp();
         tc_fence_after();
         if (any) {
@@ -636,9 +680,6 @@ __device__ __forceinline__ void run_rows_tc(const SharedDecode& p, const Layout&
           tmem_ld32(t_s, s);
           tmem_ld32(t_s + 32, s + 32);
           tmem_wait_ld();
-          // (a negative scale turns the order round: the maximum is taken of what is scaled)
-#pragma unroll
-          for (int i = 0; i < kTcKeys; ++i) s[i] *= scale;
           const int valid = part.t1 - part.t0 - j * kTcKeys;
           if (valid < kTcKeys) {
 #pragma unroll
@@ -647,74 +688,98 @@ __device__ __forceinline__ void run_rows_tc(const SharedDecode& p, const Layout&
           float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
           for (int i = 4; i < kTcKeys; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
-          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
           float f = 1.f;
           if (top > m + kSlack) {
             f = exp2_of(m - top);
             m = top;
             l *= f;
           }
-          const float off = (m == -INFINITY ? 0.f : m) - kLift<T>;
-          float sum[2] = {0.f, 0.f};
+          const float off = kLift<T> - (m == -INFINITY ? 0.f : m);
+          const unsigned long long mul = pair_of(scale, scale), add = pair_of(off, off);
+          unsigned long long sum[2] = {pair_of(0.f, 0.f), pair_of(0.f, 0.f)};
 #pragma unroll
           for (int i = 0; i < kTcKeys; i += 32) {
             uint32_t parts[3][16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              const float a = exp2_of(s[i + 2 * e] - off), b = exp2_of(s[i + 2 * e + 1] - off);
-              sum[0] += a;
-              sum[1] += b;
-              split_weights<T>(a, b, 1.f, parts[0][e], parts[1][e], parts[2][e]);
+              float a, b;
+              halves_of(fma_pair(pair_of(s[i + 2 * e], s[i + 2 * e + 1]), mul, add), a, b);
+              a = exp2_of(a);
+              b = exp2_of(b);
+              sum[e & 1] = add_pair(sum[e & 1], pair_of(a, b));
+              cut_weights<T>(a, b, parts[0][e], parts[1][e], parts[2][e]);
             }
 #pragma unroll
             for (int w = 0; w < kParts<T>; ++w) tmem_st16(t_s + w * 32 + i / 2, parts[w]);
           }
-          l += sum[0] + sum[1];
-          if (j > 0 && __any_sync(0xffffffffu, f != 1.f)) {
-            wait(bar.products, (c - 1) & 1);                   // O holds the products so far
+          float la, lb;
+          halves_of(add_pair(sum[0], sum[1]), la, lb);
+          l += la + lb;
+          if (j > 1 && __any_sync(0xffffffffu, f != 1.f)) {
+            wait(bar.products[odd], (k - 1) & 1);              // the output holds the products so far
             __syncwarp();
             tc_fence_after();
             for (int i = 0; i < kDim; i += 32) {
               float o[32];
-              tmem_ld32(tmem + kTcOut + lanes + i, o);
+              tmem_ld32(t_o + i, o);
               tmem_wait_ld();
 #pragma unroll
               for (int e = 0; e < 32; ++e) o[e] *= f;
-              tmem_st16(tmem + kTcOut + lanes + i, reinterpret_cast<const uint32_t*>(o));
-              tmem_st16(tmem + kTcOut + lanes + i + 16, reinterpret_cast<const uint32_t*>(o + 16));
+              tmem_st16(t_o + i, reinterpret_cast<const uint32_t*>(o));
+              tmem_st16(t_o + i + 16, reinterpret_cast<const uint32_t*>(o + 16));
             }
           }
           tmem_wait_st();
         }
+        ++k;
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_addr(&bar.weights[c & 1]));
+        if (lane == 0) mbar_arrive(smem_addr(&bar.weights[tile & 1]));
       }
+      c += tiles;
+      if (odd) {
+        bar.m[r] = m;
+        bar.l[r] = l;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_addr(&bar.odd));
+        continue;
+      }
+      // the even tiles' warps join both
+      wait(bar.odd, n & 1);
       wait(bar.outputs, n & 1);
       __syncwarp();
       tc_fence_after();
       if (!any) continue;
+      const float m1 = bar.m[r], both = fmaxf(m, m1);
+      const float f0 = m == -INFINITY ? 0.f : exp2_of(m - both), f1 = m1 == -INFINITY ? 0.f : exp2_of(m1 - both);
+      l = l * f0 + bar.l[r] * f1;
       const bool mine = there && at.common[min(seq, p.seqs - 1)] > 0;      // (otherwise it reads all of its keys by itself)
       const size_t to = ((size_t)seq * p.heads + part.kvh * ratio + row % ratio) * p.parts + part.index;
       bool finite = true;
       for (int i = 0; i < kDim; i += 32) {
-        float o[32];
-        tmem_ld32(tmem + kTcOut + lanes + i, o);
+        float o[32], o1[32];
+        tmem_ld32(t_o + i, o);
+        if (tiles > 1) tmem_ld32(t_o + kDim + i, o1);
         tmem_wait_ld();
         if (mine) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            finite = finite && isfinite(o[e]) && isfinite(o[e + 1]) && isfinite(o[e + 2]) && isfinite(o[e + 3]);
-            *reinterpret_cast<float4*>(p.partial + to * kDim + i + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          for (int e = 0; e < 32; ++e) {
+            o[e] *= f0;
+            if (tiles > 1) o[e] += o1[e] * f1;
+            finite = finite && isfinite(o[e]);
           }
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            *reinterpret_cast<float4*>(p.partial + to * kDim + i + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
         }
       }
-      if (mine) p.ml[to] = make_float2(m, l);
-      uint32_t again = __ballot_sync(0xffffffffu, !finite);
+      if (mine) p.ml[to] = make_float2(both, l);
+      uint32_t again = __ballot_sync(0xffffffffu, !finite && l == l);      // (a sum that is NaN stays one)
       __syncwarp();
       for (; again; again &= again - 1) {
         const int from = __ffs(again) - 1;
-        const float4 v = sum_plainly<T>(p, part, __shfl_sync(0xffffffffu, row, from), __shfl_sync(0xffffffffu, m, from));
+        const float4 v = sum_plainly<T>(p, part, __shfl_sync(0xffffffffu, row, from), __shfl_sync(0xffffffffu, both, from));
         const unsigned long long place = __shfl_sync(0xffffffffu, (unsigned long long)to, from);
         *reinterpret_cast<float4*>(p.partial + place * kDim + lane * 4) = v;
       }
@@ -783,9 +848,10 @@ shared_decode_kernel(const __grid_constant__ SharedDecode p, const __grid_consta
           mbar_init(smem_addr(&s_tc.scores[i]), 1);
           mbar_init(smem_addr(&s_tc.weights[i]), 4);
         }
-        mbar_init(smem_addr(&s_tc.products), 1);
+        for (int i = 0; i < 2; ++i) mbar_init(smem_addr(&s_tc.products[i]), 1);
         mbar_init(smem_addr(&s_tc.queries), 4);
         mbar_init(smem_addr(&s_tc.outputs), 1);
+        mbar_init(smem_addr(&s_tc.odd), 4);
       }
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
       fence_proxy_async();

@@ -277,3 +277,73 @@ def test_refusals():
         wide.run()
     empty = ops.shared_attention_decode(b.qkv[:0], b.k, b.v, i32(b.tables)[:0], i32([]), i32([]), i32([]), 0, 0, 8, 4, 16, SCALE)
     assert empty.shape == (0, 1024)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("size,heads,kvh", [(5, 8, 2), (9, 8, 1), (40, 4, 1)])
+@pytest.mark.parametrize("key", [0, 63, 64, 141, 149, 155])
+def test_infinities_among_the_values_of_many_rows(key, size, heads, kvh, dtype):
+    """The same with more rows than eight, sixteen and sixty-four, over three tiles of 64 keys."""
+    b = Batch([size, 1], [150, 20], [6] * (size + 1), heads, kvh, dtype, seed=key)
+    b.k *= 0.02
+    for s in range(size):
+        b.v[b.slot(s, key), :, 7], b.v[b.slot(s, key), :, 12] = float("inf"), float("-inf")
+    out = b.run()
+    for s in range(size):
+        want = b.want(s)
+        bad = torch.isinf(want)
+        assert int(bad.sum()) == 2 * heads and torch.equal(out[s].double()[bad], want[bad])
+        err = (out[s].double()[~bad] - want[~bad]).norm() / want[~bad].norm()
+        assert err <= TOL[dtype]
+
+
+@pytest.mark.parametrize("block", [16, 32, 5])
+@pytest.mark.parametrize("size,heads,kvh", [(3, 4, 4), (4, 8, 2), (9, 8, 1), (33, 8, 2)])
+def test_nan_behind_the_end_of_many_rows(size, heads, kvh, block):
+    """Shared lengths that end inside a tile, a box and a page, with NaN in every row of the cache that is not held."""
+    shared = [70, 1, 64, 129, 177]
+    b = Batch([size] * 5, shared, [i % 20 for i in range(5 * size)], heads, kvh, torch.bfloat16, block=block, seed=size)
+    want = b.run()
+    b.check(want)
+    used = {b.slot(s, t) for s in range(5 * size) for t in range(b.lens[s])}
+    free = torch.tensor([r for r in range(b.k.shape[0]) if r not in used], device="cuda")
+    b.k[free], b.v[free] = float("nan"), float("nan")
+    assert torch.equal(b.run(), want)
+
+
+@pytest.mark.parametrize("size,heads,kvh", [(3, 2, 2), (5, 8, 2), (9, 8, 1)])
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 1e-3, 5.0])
+def test_scales(scale, size, heads, kvh):
+    from deltazip_b200 import ops
+    b = Batch([size, 2], [200, 30], [9] * (size + 2), heads, kvh, torch.float16, seed=3)
+    out = ops.shared_attention_decode(b.qkv, b.k, b.v, i32(b.tables), i32(b.lens), i32(b.starts), i32(b.shared), size, 200, heads, kvh,
+                                      16, scale)
+    global SCALE
+    was, SCALE = SCALE, scale
+    try:
+        b.check(out)
+    finally:
+        SCALE = was
+
+
+@pytest.mark.parametrize("sizes", [[9], [12, 3, 16], [16] * 40])
+def test_parts_of_every_length(sizes):
+    """Groups of more than 16 rows whose parts have one, two and many tiles of 64 keys; a CTA takes several parts."""
+    for longest in (1, 64, 65, 128, 700, 5000):
+        rng = random.Random(longest)
+        shared = [rng.randint(1, longest) for _ in sizes]
+        if len(sizes) > 3:
+            shared = [min(n, 300) for n in shared]
+        b = Batch(sizes, shared, [rng.randint(0, 5) for _ in range(sum(sizes))], 8, 2, torch.float16, seed=longest)
+        b.check(b.run())
+
+
+def test_large_scores_move_the_maximum():
+    """Scores that rise along the keys, by more than a step of the running maximum from tile to tile."""
+    for size, heads, kvh in ((2, 2, 2), (4, 8, 2), (9, 8, 1)):
+        b = Batch([size], [900], [40] * size, heads, kvh, torch.bfloat16, seed=size)
+        for s in range(size):
+            at = torch.tensor([b.slot(s, t) for t in range(b.lens[s])], device="cuda")
+            b.k[at] = (b.k[at].float() * 0.05 + torch.linspace(0, 6, len(at), device="cuda")[:, None, None] *
+                       b.qkv[0, :128].float().sign()[None, None]).to(torch.bfloat16)
+        b.check(b.run())
