@@ -49,7 +49,8 @@ constexpr int kWarps = 12, kThreads = kWarps * 32, kStages = 2, kTile = 16;    /
 constexpr int kRowBytes = kDim * 2, kHalfStage = kTile * kRowBytes, kStageBytes = 2 * kHalfStage;
 constexpr int kRingBytes = kStages * kStageBytes;
 constexpr int kMaxSeqs = 1024;           // also groups: what the layout of the parts takes of shared memory
-constexpr int kMaxParts = 64;            // of a row
+constexpr int kMaxParts = 32;            // of a row's shared keys, and of its own
+constexpr int kLeastSpan = 32;           // keys of a part at least
 constexpr int kEight = 8;                // rows that leave half of an MMA's to the weights' parts
 
 struct SharedDecode {
@@ -70,7 +71,7 @@ struct SharedDecode {
   float scale;
   int max_group, max_shared;
   int team;                              // warps that take shared keys together (1, 2, 4)
-  int least, parts;                      // keys of a part at least, parts of a row at most
+  int parts;                             // of a row at most
   float* partial;                        // [sequences, heads, parts, 128]
   float2* ml;                            // [sequences, heads, parts] maximum and sum
   int* common;                           // [sequences] keys that a sequence reads with its group
@@ -788,12 +789,12 @@ __device__ __forceinline__ void run_rows_tc(const SharedDecode& p, const Layout&
 }
 
 // Keys of a part, of which `total` (over heads and blocks of rows) are dealt to `teams`: n parts for each, n being the
-// smallest number that leaves them idle for less than a tenth of the time, or the best there is.  parts(span): how many there
-// are.  Warp `n` - 1 of those that look for it tries n.
+// smallest number that leaves them idle for less than a tenth of the time, or the best there is.  A row of `longest` keys has
+// kMaxParts at most.  parts(span): how many there are.  Warp `n` - 1 of those that look for it tries n.
 constexpr int kTries = kWarps / 2;
 template <typename F>
-__device__ __forceinline__ void try_span(const SharedDecode& p, float total, int teams, int n, int step, float* tried, F parts) {
-  const int least = (p.least + step - 1) / step * step;
+__device__ __forceinline__ void try_span(float total, int longest, int teams, int n, int step, float* tried, F parts) {
+  const int least = (max(kLeastSpan, (longest + kMaxParts - 1) / kMaxParts) + step - 1) / step * step;
   int span = 0, count = 0;
   for (int again = 0; again < 3; ++again) {
     const float want = again ? span * 1.0625f + 1.f : total / (float)(teams * n);     // (the last try took too many parts)
@@ -819,7 +820,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 shared_decode_kernel(const __grid_constant__ SharedDecode p, const __grid_constant__ CUtensorMap map_k,
                      const __grid_constant__ CUtensorMap map_v) {
   extern __shared__ uint8_t dynamic[];
-  __shared__ int s_warp[kWarps], s_abort;
+  __shared__ int s_warp[kWarps], s_most[2][kWarps], s_abort;
   __shared__ float s_total[2][kWarps], s_tried[2][2 * kTries];
   __shared__ uint64_t s_full[kWarps * kStages];
   __shared__ TcBarriers s_tc;
@@ -875,6 +876,7 @@ shared_decode_kernel(const __grid_constant__ SharedDecode p, const __grid_consta
   };
   auto blocks_of = [&](int g) { return (members(g) * ratio + block_rows - 1) / block_rows; };
   float shared_total = 0.f, own_total = 0.f;
+  int shared_most = 0, own_most = 0;
   for (int seq = threadIdx.x; seq < p.seqs; seq += kThreads) {
     int common = 0;                      // a sequence that is shorter than its group's shared keys reads all of its own by itself
     if (p.groups > 0) {
@@ -886,6 +888,7 @@ shared_decode_kernel(const __grid_constant__ SharedDecode p, const __grid_consta
     at.common[seq] = common;
     at.own[seq] = own;
     own_total += (float)own;
+    own_most = max(own_most, own);
     if (blockIdx.x == 0) p.common[seq] = common;
   }
   for (int g = threadIdx.x; g < p.groups; g += kThreads) {
@@ -895,25 +898,34 @@ shared_decode_kernel(const __grid_constant__ SharedDecode p, const __grid_consta
     at.source[g] = source;
     at.shared[g] = source < first + n ? at.keys[g] : 0;
     shared_total += (float)at.shared[g] * (float)blocks_of(g);
+    shared_most = max(shared_most, at.shared[g]);
   }
   shared_total = warp_sum(shared_total);
   own_total = warp_sum(own_total);
-  if (lane == 0) { s_total[0][warp] = shared_total; s_total[1][warp] = own_total; }
+  shared_most = __reduce_max_sync(0xffffffffu, shared_most);
+  own_most = __reduce_max_sync(0xffffffffu, own_most);
+  if (lane == 0) {
+    s_total[0][warp] = shared_total;
+    s_total[1][warp] = own_total;
+    s_most[0][warp] = shared_most;
+    s_most[1][warp] = own_most;
+  }
   __syncthreads();
   {
     const int kind = warp / kTries, n = warp % kTries + 1;
     const float total = warp_sum(lane < kWarps ? s_total[kind][lane] : 0.f) * (float)p.kv_heads;
+    const int longest = __reduce_max_sync(0xffffffffu, lane < kWarps ? s_most[kind][lane] : 0);
     auto over = [&](int many, auto count) {                    // (numbers beyond any launch's are cut off)
       float sum = 0.f;
       for (int i = lane; i < many; i += 32) sum += (float)count(i);
       return (int)fminf(warp_sum(sum) * (float)p.kv_heads, 1e9f);
     };
     if (kind == 0)
-      try_span(p, total, shared_teams, n, kShared == kOnTc ? kTcKeys : p.team * kTile, s_tried[0], [&](int span) {
+      try_span(total, longest, shared_teams, n, kShared == kOnTc ? kTcKeys : p.team * kTile, s_tried[0], [&](int span) {
         return over(p.groups, [&](int g) { return (at.shared[g] + span - 1) / span * blocks_of(g); });
       });
     else
-      try_span(p, total, gridDim.x * kWarps, n, kTile, s_tried[1], [&](int span) {
+      try_span(total, longest, gridDim.x * kWarps, n, kTile, s_tried[1], [&](int span) {
         return over(p.seqs, [&](int seq) { return (at.own[seq] + span - 1) / span; });
       });
   }
@@ -993,17 +1005,15 @@ __global__ void __launch_bounds__(256) shared_join_kernel(SharedDecode p) {
 }
 
 struct Plan {
-  int team, least, parts;
+  int team, parts;
 };
 Plan plan(int num_seqs, int max_group, int max_keys, int heads, int kv_heads) {
   Plan r;
   const int64_t rows = (int64_t)(max_group < num_seqs ? max_group : num_seqs) * (heads / kv_heads);
   r.team = rows <= kRows ? 1 : rows <= 2 * kRows ? 2 : 4;
-  // no part has fewer keys than this (64 of shared keys on tcgen05: it is rounded up there), so that a row has kMaxParts at
-  // most, whatever its lengths are
-  const int step = r.team * kTile, some = (max_keys + kMaxParts - 5) / (kMaxParts - 4), least = some > 32 ? some : 32;
-  r.least = (least + step - 1) / step * step;
-  r.parts = max_keys / r.least + 3;
+  // (own keys count from a multiple of 16)
+  r.parts = max_keys / kLeastSpan + 3;
+  if (r.parts > 2 * kMaxParts) r.parts = 2 * kMaxParts;
   return r;
 }
 struct Scratch {
@@ -1087,7 +1097,7 @@ int dz_shared_attention_decode(const dz_shared_attention_args* a, void* stream) 
   const SharedDecode p = {a->qkv, a->q_row_stride, a->out, a->k_cache, a->v_cache, (uint32_t)(a->cache_rows - 1),
                           (uint32_t)((a->cache_rows - 1) / a->block_size), a->block_tables, a->table_width,
                           a->block_size, magic, 31 + log, a->seq_lens, a->group_starts, a->shared_lens, a->num_groups, a->num_seqs, a->q_heads,
-                          a->kv_heads, a->scale, a->max_group, a->max_shared, r.team, r.least, r.parts,
+                          a->kv_heads, a->scale, a->max_group, a->max_shared, r.team, r.parts,
                           reinterpret_cast<float*>(ws), reinterpret_cast<float2*>(ws + at.ml), reinterpret_cast<int*>(ws + at.common), reinterpret_cast<int*>(ws + at.spans), a->status};
   cudaStream_t st = (cudaStream_t)stream;
   const int rows = a->num_seqs * a->q_heads;
