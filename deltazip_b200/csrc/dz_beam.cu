@@ -140,11 +140,16 @@ __global__ void __launch_bounds__(kThreads, 4) beam_rows_kernel(BeamRows p) {
   for (int piece = 0, from = base; from < end; ++piece, from += kPiece) {
     load(from + kPiece, (piece + 1) & 1);
     cp_async_wait<1>();
-    const uint8_t* ring = s_ring + (piece & 1) * (kPiece * sizeof(T));
+    T* ring = reinterpret_cast<T*>(s_ring) + (piece & 1) * kPiece;
+    if (from < skip || from + kPiece > end) {                  // the row's first or last piece
+#pragma unroll 1
+      for (int j = 0; j < E; ++j)
+        if (from + place(j) < skip || from + place(j) >= end) ring[place(j)] = Cvt<T>::from(-INFINITY);
+    }
     float x[E];
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
-      const uint4 v = *reinterpret_cast<const uint4*>(ring + (j * kThreads + tid) * 16);
+      const uint4 v = *reinterpret_cast<const uint4*>(ring + (j * kThreads + tid) * W);
       const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -156,11 +161,6 @@ __global__ void __launch_bounds__(kThreads, 4) beam_rows_kernel(BeamRows p) {
           x[j * 8 + 2 * e + 1] = f.y;
         }
       }
-    }
-    if (from < skip || from + kPiece > end) {                  // the row's first or last piece
-#pragma unroll
-      for (int j = 0; j < E; ++j)
-        if (from + place(j) < skip || from + place(j) >= end) x[j] = -INFINITY;
     }
     float eight[E / 8], mine = -INFINITY;                      // maxima of eight (fmaxf passes over NaN)
 #pragma unroll
@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(kThreads, 4) beam_rows_kernel(BeamRows p) {
         int at = have + atomicAdd(&s_new[piece % 3], __popc(reach));
         for (; reach && at < kRoom; reach &= reach - 1) {      // few
           const int i = place(__ffs(reach) - 1);
-          s_found[at++] = key_of(Cvt<T>::one(reinterpret_cast<const T*>(ring)[i]), from + i);
+          s_found[at++] = key_of(Cvt<T>::one(ring[i]), from + i);
         }
       }
     }
@@ -252,10 +252,10 @@ __global__ void __launch_bounds__(kThreads, 4) beam_rows_kernel(BeamRows p) {
       for (; taken < p.k; ++taken) {
         if (again) {                                           // the thread's best behind the last one taken
           next = kept < last ? kept : 0;
-#pragma unroll
+#pragma unroll 1
           for (int j = 0; j < E; ++j) {
             const int at = from + place(j);
-            const uint64_t key = key_of(fmaxf(x[j], -INFINITY), at);      // NaN counts as -inf
+            const uint64_t key = key_of(fmaxf(Cvt<T>::one(ring[place(j)]), -INFINITY), at);      // NaN counts as -inf
             if (at >= skip && at < end && key < last && key > next) next = key;
           }
           again = false;
@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(kThreads) beam_groups_kernel(BeamGroups p) {
 }
 
 // How rows are cut: spans of pieces of `elements` per thread.  Small pieces, one a span, spread few rows over the SMs; where
-// there are enough of the large ones, spans are as long as four CTAs on every SM leave them.
+// there are enough of the large ones, spans are as long as to leave one round of four CTAs on every SM.
 struct Cut {
   int elements, pieces, splits;
 };
@@ -498,7 +498,7 @@ Cut cut_rows(int rows, int vocab, int dtype) {
   if ((int64_t)rows * c.splits < 148) {
     c = {kSmall, 1, count(kSmall)};
   } else {
-    const int want = (most + rows - 1) / rows;
+    const int want = rows < most ? most / rows : 1;
     if (want < c.splits) {
       c.pieces = (c.splits + want - 1) / want;
       c.splits = (c.splits + c.pieces - 1) / c.pieces;
