@@ -97,7 +97,7 @@ __device__ __noinline__ void copy_together(uint8_t* base, int64_t page_bytes, in
     default: { using V = uint8_t; CALL; break; }          \
   }
 
-__global__ void __launch_bounds__(kThreads, 3) copy_pages_kernel(CopyPages p) {
+__global__ void __launch_bounds__(kThreads, 2) copy_pages_kernel(CopyPages p) {
   extern __shared__ __align__(16) int smem[];
   __shared__ int s_warp[kThreads / 32];
   int* s_page = smem;                                          // [slots] a destination, -1: none
@@ -260,7 +260,7 @@ int dz_copy_pages(const int64_t* pools, int num_pools, int num_pages, int page_r
   const size_t smem = ((size_t)2 * slots + 3 * pairs + num_pools + 1) * 4;
   // no more CTAs than items, in the form that has more of them
   const int64_t items = (page_units / kItem + num_pools) * pairs;
-  const int per_sm = smem <= 70 * 1024 ? 3 : smem <= 100 * 1024 ? 2 : 1;
+  const int per_sm = smem <= 100 * 1024 ? 2 : 1;
   const int grid = (int)(items < 148 * per_sm ? items : 148 * per_sm);
   DZ_CUDA_OK(allow_smem(copy_pages_kernel, smem));
   DZ_CUDA_OK(launch_ex(copy_pages_kernel, dim3(grid), dim3(kThreads), smem, 1, (cudaStream_t)stream, p));
