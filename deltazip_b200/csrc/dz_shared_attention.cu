@@ -132,32 +132,31 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes)
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
-// Running sums of count(i), i < n, in front of each i and at sums[n]; count may read sums[i].  Every thread of the block
-// calls it.
-template <typename F>
-__device__ __forceinline__ void lay_out(int n, int* sums, int* warp_sums, F count) {
+// Turns a[i] (i < n) and b[i] (i < m) into running sums in front of each, the whole at a[n] and b[m].  Every thread of the
+// block calls it.
+__device__ __forceinline__ void lay_out(int n, int* a, int m, int* b, int2* warp_sums) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int before = 0;
-  for (int i0 = 0; i0 < n; i0 += kThreads) {
-    const int i = i0 + threadIdx.x, c = i < n ? count(i) : 0;
-    int upto = c;
+  int2 before = make_int2(0, 0);
+  for (int i0 = 0; i0 < max(n, m); i0 += kThreads) {
+    const int i = i0 + threadIdx.x;
+    const int2 c = make_int2(i < n ? a[i] : 0, i < m ? b[i] : 0);
+    int2 upto = c;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += up;
+      const int x = __shfl_up_sync(0xffffffffu, upto.x, o), y = __shfl_up_sync(0xffffffffu, upto.y, o);
+      if (lane >= o) { upto.x += x; upto.y += y; }
     }
     if (lane == 31) warp_sums[warp] = upto;
     __syncthreads();
-    int ahead = before, all = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      ahead += w < warp ? warp_sums[w] : 0;
-      all += warp_sums[w];
-    }
-    if (i < n) sums[i] = ahead + upto - c;
-    before += all;
+    const int2 mine = lane < kWarps ? warp_sums[lane] : make_int2(0, 0);
+    const int2 ahead = make_int2(__reduce_add_sync(0xffffffffu, lane < warp ? mine.x : 0), __reduce_add_sync(0xffffffffu, lane < warp ? mine.y : 0));
+    if (i < n) a[i] = before.x + ahead.x + upto.x - c.x;
+    if (i < m) b[i] = before.y + ahead.y + upto.y - c.y;
+    before.x += __reduce_add_sync(0xffffffffu, mine.x);
+    before.y += __reduce_add_sync(0xffffffffu, mine.y);
     __syncthreads();
   }
-  if (threadIdx.x == 0) sums[n] = before;
+  if (threadIdx.x == 0) { a[n] = before.x; b[m] = before.y; }
 }
 
 // A span of keys for some rows: tiles from t0 on, of which the keys t_lo <= t < t1 count.
@@ -807,11 +806,14 @@ __device__ __forceinline__ void try_span(float total, int longest, int teams, in
     tried[2 * n - 1] = ceilf((float)count / (float)teams) * (float)span;
   }
 }
-__device__ __forceinline__ int best_span(const float* tried) {
-  int best = 0;
-  for (int i = 1; i < kTries; ++i)
-    if (tried[2 * i + 1] < 0.9f * tried[2 * best + 1]) best = i;
-  return (int)tried[2 * best];
+__device__ __forceinline__ int best_span(const float (&tried)[2 * kTries]) {
+  float span = tried[0], spent = tried[1];
+#pragma unroll
+  for (int i = 1; i < kTries; ++i) {
+    const float s = tried[2 * i], t = tried[2 * i + 1];
+    if (t < 0.9f * spent) { span = s; spent = t; }
+  }
+  return (int)span;
 }
 
 enum { kByTeams, kFewRows, kOnTc };      // how shared keys are taken
@@ -820,7 +822,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 shared_decode_kernel(const __grid_constant__ SharedDecode p, const __grid_constant__ CUtensorMap map_k,
                      const __grid_constant__ CUtensorMap map_v) {
   extern __shared__ uint8_t dynamic[];
-  __shared__ int s_warp[kWarps], s_most[2][kWarps], s_abort;
+  __shared__ int2 s_warp[kWarps];
+  __shared__ int s_most[2][kWarps], s_abort;
   __shared__ float s_total[2][kWarps], s_tried[2][2 * kTries];
   __shared__ uint64_t s_full[kWarps * kStages];
   __shared__ TcBarriers s_tc;
@@ -836,26 +839,24 @@ shared_decode_kernel(const __grid_constant__ SharedDecode p, const __grid_consta
   at.own = at.common + p.seqs;
   at.full = s_full;
   at.abort = &s_abort;
-  if (threadIdx.x == 0) {
-    s_abort = 0;
-    if (kTma) {
-      for (int i = 0; i < kWarps * kStages; ++i) mbar_init(smem_addr(s_full + i), 1);
-      if (kShared == kOnTc) {
-        for (int i = 0; i < kTcStages; ++i) {
-          mbar_init(smem_addr(&s_tc.full[i]), 3);
-          mbar_init(smem_addr(&s_tc.empty[i]), 1);
-        }
-        for (int i = 0; i < 2; ++i) {
-          mbar_init(smem_addr(&s_tc.scores[i]), 1);
-          mbar_init(smem_addr(&s_tc.weights[i]), 4);
-        }
-        for (int i = 0; i < 2; ++i) mbar_init(smem_addr(&s_tc.products[i]), 1);
-        mbar_init(smem_addr(&s_tc.queries), 4);
-        mbar_init(smem_addr(&s_tc.outputs), 1);
-        mbar_init(smem_addr(&s_tc.odd), 4);
+  if (threadIdx.x == 0) s_abort = 0;
+  if (kTma) {
+    if (threadIdx.x < kWarps * kStages) mbar_init(smem_addr(s_full + threadIdx.x), 1);
+    if (kShared == kOnTc) {
+      const int i = (int)threadIdx.x - 32;
+      if (i >= 0 && i < kTcStages) { mbar_init(smem_addr(&s_tc.full[i]), 3); mbar_init(smem_addr(&s_tc.empty[i]), 1); }
+      if (i >= 8 && i < 10) {
+        mbar_init(smem_addr(&s_tc.scores[i - 8]), 1);
+        mbar_init(smem_addr(&s_tc.weights[i - 8]), 4);
+        mbar_init(smem_addr(&s_tc.products[i - 8]), 1);
       }
+      if (i == 10) { mbar_init(smem_addr(&s_tc.queries), 4); mbar_init(smem_addr(&s_tc.outputs), 1); mbar_init(smem_addr(&s_tc.odd), 4); }
+    }
+    if (threadIdx.x < 64) {
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
       fence_proxy_async();
+    }
+    if (threadIdx.x == 64) {
       asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
       asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
     }
@@ -917,24 +918,27 @@ shared_decode_kernel(const __grid_constant__ SharedDecode p, const __grid_consta
     const int longest = __reduce_max_sync(0xffffffffu, lane < kWarps ? s_most[kind][lane] : 0);
     auto over = [&](int many, auto count) {                    // (numbers beyond any launch's are cut off)
       float sum = 0.f;
-      for (int i = lane; i < many; i += 32) sum += (float)count(i);
+      for (int i = lane; i < many; i += 32) sum += count(i);
       return (int)fminf(warp_sum(sum) * (float)p.kv_heads, 1e9f);
     };
     if (kind == 0)
       try_span(total, longest, shared_teams, n, kShared == kOnTc ? kTcKeys : p.team * kTile, s_tried[0], [&](int span) {
-        return over(p.groups, [&](int g) { return (at.shared[g] + span - 1) / span * blocks_of(g); });
+        const float one = 1.f / (float)span;                   // (a part more or less does not matter here)
+        return over(p.groups, [&](int g) { return ceilf((float)at.shared[g] * one) * (float)blocks_of(g); });
       });
     else
       try_span(total, longest, gridDim.x * kWarps, n, kTile, s_tried[1], [&](int span) {
-        return over(p.seqs, [&](int seq) { return (at.own[seq] + span - 1) / span; });
+        const float one = 1.f / (float)span;
+        return over(p.seqs, [&](int seq) { return ceilf((float)at.own[seq] * one); });
       });
   }
   __syncthreads();
   at.shared_span = best_span(s_tried[0]);
   at.own_span = best_span(s_tried[1]);
   if (blockIdx.x == 0 && threadIdx.x == 0) { p.spans[0] = at.shared_span; p.spans[1] = at.own_span; }
-  lay_out(p.groups, at.shared, s_warp, [&](int g) { return (at.shared[g] + at.shared_span - 1) / at.shared_span * blocks_of(g); });
-  lay_out(p.seqs, at.own, s_warp, [&](int seq) { return (at.own[seq] + at.own_span - 1) / at.own_span; });
+  for (int g = threadIdx.x; g < p.groups; g += kThreads) at.shared[g] = (at.shared[g] + at.shared_span - 1) / at.shared_span * blocks_of(g);
+  for (int seq = threadIdx.x; seq < p.seqs; seq += kThreads) at.own[seq] = (at.own[seq] + at.own_span - 1) / at.own_span;
+  lay_out(p.groups, at.shared, p.seqs, at.own, s_warp);        // (each thread begins with what it has written)
   __syncthreads();
 
   uint32_t used = 0;
