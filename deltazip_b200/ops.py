@@ -1072,6 +1072,9 @@ class PagePools:
         self.tensors = [t for t in tensors if t.numel()]        # kept: the table holds their addresses
         if len({t.device for t in self.tensors}) > 1:
             raise ValueError("all pools are on one GPU")
+        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in self.tensors)
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError("no two pools lie in the same memory")
         entries, self.page_units = [], 0
         for t in self.tensors:
             row = t.numel() // t.shape[0] * t.element_size()

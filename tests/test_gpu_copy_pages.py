@@ -176,6 +176,6 @@ def test_refusals():
     with pytest.raises(DeltaZipError):
         ops.copy_pages(handle, i32([0] * n), i32([1] * n))
     for tensors, per in (([pool], 3), ([pool], 0), ([pool.t()], 4), ([pool, pool[:8]], 4), ([pool.cpu()], 4),
-                         ([torch.zeros((), device="cuda")], 1)):
+                         ([torch.zeros((), device="cuda")], 1), ([pool, pool], 4), ([pool[:8], pool[4:12]], 4)):
         with pytest.raises(ValueError):
             ops.PagePools(tensors, per)
