@@ -12,6 +12,12 @@
 //   groups  a CTA joins its rows' maxima and sums, takes the entries of its spans' lists into registers, searches for a score
 //           that k to about 2 k of them reach, and ranks those by counting -- or, where too many are equal, takes the best
 //           one after the other.
+// Bound: the logits' bytes, and for a few rows the two launches.  A piece costs a CTA as much again as its loads: three
+// instructions of an exponential an element, the maxima, and what it takes to collect and rank what reaches the floor, which
+// is why the floor rises with every piece (73 us before, 57 with it, as both were then).  Measured from a cold cache: 284 rows of
+// 131072 tokens in bf16, groups of up to 16, k = 32 (74 MB, 11.4 us at the copy bandwidth): 47 us, 37 of them before the second
+// launch; 128 rows of 32000 floats, k = 16: 21 us; 4 rows, k = 8: 14.  (The first with every thread naming its best, k times, as
+// the only way: 180 us in a row of calls, where it takes 42.)
 // Sums are 32-bit within a thread's piece (at most 32 terms) and 64-bit beyond, and so are the scores that rows are compared by:
 // beams come close to one another, and which is ahead is not to hang on a rounding.
 #include "dz_elem.cuh"
@@ -21,7 +27,9 @@ namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMaxKeep = 128;
-constexpr int kSmall = 8;                // elements of a thread and piece; larger pieces: 64 bytes
+template <typename T>
+constexpr int kElements = 64 / sizeof(T);                      // of a thread and piece
+constexpr int kListed = 2048, kListsAtATime = 256;             // entries and lists that the second launch takes at a time
 constexpr int kRoom = 640;               // logits that are ranked by counting
 constexpr float kToLog2 = 1.4426950408889634f;                 // as a float, which is what the exponents are taken with
 constexpr double kLn2 = 0.6931471805599453;
@@ -101,9 +109,9 @@ __device__ __forceinline__ void rank_found(const uint64_t* found, int n, F use) 
 
 // A thread has E elements of a piece, in loads of 16 bytes: rows may start anywhere, so a row counts from the 16-byte boundary
 // at or before its first element, and what lies before it or behind its end is left out.
-template <typename T, int E>
+template <typename T>
 __global__ void __launch_bounds__(kThreads, 4) beam_rows_kernel(BeamRows p) {
-  constexpr int kPiece = kThreads * E, W = 16 / sizeof(T), kLoads = E / W;
+  constexpr int E = kElements<T>, kPiece = kThreads * E, W = 16 / sizeof(T), kLoads = E / W;
   extern __shared__ __align__(16) uint8_t s_ring[];            // two pieces
   __shared__ uint64_t s_found[kRoom], s_best_k[kMaxKeep];
   __shared__ __align__(16) uint32_t s_max[kThreads];
@@ -324,7 +332,7 @@ struct BeamGroups {
 };
 
 __global__ void __launch_bounds__(kThreads) beam_groups_kernel(BeamGroups p) {
-  constexpr int kEntries = 8, kBatch = kThreads * kEntries;   // entries of the lists at a time
+  constexpr int kEntries = kListed / kThreads;   // entries of the lists at a time
   __shared__ Key s_kept[kMaxKeep], s_found[kRoom], s_best[2][kWarps];       // kept: best first; place: entry of the group's lists
   __shared__ int s_kept_token[kMaxKeep], s_found_token[kRoom], s_count, s_part[2][kWarps];
   __shared__ double s_base[kThreads];                         // the score of a row's largest logit
@@ -334,7 +342,7 @@ __global__ void __launch_bounds__(kThreads) beam_groups_kernel(BeamGroups p) {
   pdl_wait();
   pdl_launch();
   const int first = min(max(p.starts[g], 0), p.rows), last = min(max(p.starts[g + 1], first), p.rows);
-  const int lists = (last - first) * p.splits, batch = min(kBatch / p.k, kThreads);      // lists at a time
+  const int lists = (last - first) * p.splits, batch = min(kListed / p.k, kListsAtATime);      // lists at a time
   int kept = 0;
   for (int l0 = 0; l0 < lists; l0 += batch) {
     const int n = min(batch, lists - l0), r0 = l0 / p.splits, r1 = (l0 + n - 1) / p.splits;
@@ -485,26 +493,31 @@ __global__ void __launch_bounds__(kThreads) beam_groups_kernel(BeamGroups p) {
   }
 }
 
-// How rows are cut: spans of pieces of `elements` per thread.  Small pieces, one a span, spread few rows over the SMs; where
-// there are enough of the large ones, spans are as long as to leave one round of four CTAs on every SM.
+// How rows are cut into spans of pieces, whose lists the second launch joins: a piece more takes a CTA 3 us, and 2048 entries
+// more of a group's lists take the second launch 9, one after the other; no more CTAs than four on every SM.  (32 rows of 131072
+// 16-bit tokens in one group, k = 64: a span of one piece 160 us, this rule 45; 32000 floats 88 and 39.  Pieces of eight elements a
+// thread where there are few rows: 14 to 16 us as with these up to 8 rows of 32000 tokens, with more 38 for 20 and 150 for 51.)
 struct Cut {
-  int elements, pieces, splits;
+  int pieces, splits;
 };
-Cut cut_rows(int rows, int vocab, int dtype) {
-  const int large = dtype == DZ_DTYPE_F32 ? 16 : 32, most = 148 * 4;
-  const int longest = vocab + 16 / (dtype == DZ_DTYPE_F32 ? 4 : 2) - 1;       // of a row counted from a 16-byte boundary
-  auto count = [&](int e) { return (longest + kThreads * e - 1) / (kThreads * e); };
-  Cut c = {large, 1, count(large)};
-  if ((int64_t)rows * c.splits < 148) {
-    c = {kSmall, 1, count(kSmall)};
-  } else {
-    const int want = rows < most ? most / rows : 1;
-    if (want < c.splits) {
-      c.pieces = (c.splits + want - 1) / want;
-      c.splits = (c.splits + c.pieces - 1) / c.pieces;
+int pieces_of(int vocab, int dtype) {    // of a row counted from a 16-byte boundary
+  const int size = dtype == DZ_DTYPE_F32 ? 4 : 2, longest = vocab + 16 / size - 1, piece = kThreads * 64 / size;
+  return (longest + piece - 1) / piece;
+}
+Cut cut_rows(int rows, int groups, int vocab, int k, int dtype) {
+  const int count = pieces_of(vocab, dtype), most = rows < 148 * 4 ? 148 * 4 / rows : 1;
+  const int64_t group = (rows + groups - 1) / groups, lists = kListed / k < kListsAtATime ? kListed / k : kListsAtATime;
+  Cut best = {count, 1};
+  int64_t least = -1;
+  for (int n = 1; n <= most && n <= count; ++n) {
+    const int pieces = (count + n - 1) / n, splits = (count + pieces - 1) / pieces;
+    const int64_t cost = 3 * pieces + 9 * ((group * splits + lists - 1) / lists);
+    if (least < 0 || cost < least) {
+      least = cost;
+      best = {pieces, splits};
     }
   }
-  return c;
+  return best;
 }
 int list_width(int k) { return (k + 3) / 4 * 4; }
 
@@ -522,10 +535,10 @@ Scratch scratch(int rows, int splits, int k) {
   return s;
 }
 
-template <typename T, int E>
+template <typename T>
 int launch_rows(const BeamRows& p, int rows, cudaStream_t st) {
-  const size_t smem = 2 * kThreads * E * sizeof(T);
-  DZ_CUDA_OK(launch_ex(beam_rows_kernel<T, E>, dim3(p.splits, rows), dim3(kThreads), smem, 1, st, p));
+  const size_t smem = 2 * kThreads * kElements<T> * sizeof(T);
+  DZ_CUDA_OK(launch_ex(beam_rows_kernel<T>, dim3(p.splits, rows), dim3(kThreads), smem, 1, st, p));
   return DZ_OK;
 }
 
@@ -538,9 +551,10 @@ extern "C" {
 
 size_t dz_beam_select_workspace_bytes(int rows, int vocab, int k) {
   if (rows <= 0 || vocab <= 0 || k <= 0 || k > kMaxKeep) return 0;
-  size_t most = 0;                                             // whatever the type
+  size_t most = 0;                                             // whatever the type and the groups
   for (int dtype : {DZ_DTYPE_F16, DZ_DTYPE_F32}) {
-    const size_t n = scratch(rows, cut_rows(rows, vocab, dtype).splits, k).total;
+    const int count = pieces_of(vocab, dtype), splits = rows < 148 * 4 ? 148 * 4 / rows : 1;
+    const size_t n = scratch(rows, splits < count ? splits : count, k).total;
     if (n > most) most = n;
   }
   return most;
@@ -556,7 +570,7 @@ int dz_beam_select(const void* logits, int64_t row_stride, int rows, int vocab, 
   if (k > kMaxKeep || rows > 65535 || vocab > (1 << 30)) return DZ_ERR_TOO_LARGE;
   const int size = dtype == DZ_DTYPE_F32 ? 4 : 2;
   if ((uintptr_t)logits % size) return DZ_ERR_ALIGNMENT;
-  const Cut cut = cut_rows(rows > 0 ? rows : 1, vocab, dtype);
+  const Cut cut = cut_rows(rows > 0 ? rows : 1, num_groups, vocab, k, dtype);
   const int splits = cut.splits;
   if ((int64_t)rows * splits * k > 0x7fffffff) return DZ_ERR_TOO_LARGE;
   uint8_t* ws = (uint8_t*)workspace;
@@ -568,7 +582,7 @@ int dz_beam_select(const void* logits, int64_t row_stride, int rows, int vocab, 
     const BeamRows p = {logits, row_stride, vocab, k, splits, cut.pieces, list_width(k), (double*)(ws + at.sums), (float2*)(ws + at.tops),
                         (float*)(ws + at.values), (int*)(ws + at.tokens)};
     int rc = DZ_OK;
-    DZ_DISPATCH(dtype, rc = cut.elements == kSmall ? launch_rows<T, kSmall>(p, rows, st) : launch_rows<T, 64 / sizeof(T)>(p, rows, st));
+    DZ_DISPATCH(dtype, rc = launch_rows<T>(p, rows, st));
     if (rc != DZ_OK) return rc;
   }
   const BeamGroups q = {group_starts, scores, (const double*)(ws + at.sums), (const float2*)(ws + at.tops),
