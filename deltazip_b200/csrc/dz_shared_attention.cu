@@ -11,7 +11,7 @@
 //
 // One CTA of twelve warps per SM stays for the whole launch.  It first lays out all parts (how long they are and how many,
 // by scans over groups and sequences in shared memory, the same in every CTA), then takes every n-th part: of shared keys as
-// a whole on tcgen05 where a group has more than 16 rows, otherwise warp by warp; then of own keys warp by warp.  A warp's
+// a whole on tcgen05 where a group has more than 16 rows and they are long, otherwise warp by warp; then of own keys warp by warp.  A warp's
 // ring of key tiles runs on from part to part, so that the end of one is not waited for.  Neighbouring parts have
 // neighbouring heads of the same cache rows, and go to different SMs.
 //
@@ -21,21 +21,26 @@
 // On tcgen05 up to 128 rows are the lanes of tensor memory, tiles are 64 keys: S = Q K^T in two buffers, a thread per row takes
 // its scores and puts the weights' parts in their place, O += P V with the parts one after the other.  Four warps do that for
 // the even tiles and four for the odd ones, each with a maximum, a sum and an output of its own, which are joined at the
-// part's end; two warps bring K and V (five stages), one issues the MMAs.  (On warp MMAs, 64 rows took two and a half times
-// the time of the cache's bytes, with four warps on all tiles 1.6 times: the softmax is what takes longest.)
+// part's end; two warps bring K and V (five stages), one issues the MMAs.  (4 groups of 64 rows,
+// 16384 keys: warp MMAs 122 us, four warps on all tiles 86, these 74; the softmax is what takes longest.)
 //
-// Warp by warp, rows are those of 16 x 8 x 16 MMAs (teams of two or four warps share key tiles, 16 rows each, where pages
-// are not whole tiles).
+// Warp by warp, rows are those of 16 x 8 x 16 MMAs (teams of two or four warps share key tiles, 16 rows each).
 //   scores   S[rows, 8 keys] += Q K^T; the order of the 128 products of a score is free, so a lane's 16-byte piece of
 //            a key row serves two MMAs as it lies.
 //   output   O[rows, 128] += P V: a weight is the sum of two (fp16) or three (bf16) 16-bit parts.  V comes transposed by
 //            ldmatrix.
+// (Eight rows in this manner and in that of more, 8 groups of 8, 32 heads: 512 keys 41 and 45 us, 4096 keys 88 both.)
 // With up to eight rows the other eight of an MMA carry the other parts (fp16: one MMA with the first and the second part;
 // bf16: two of half the first part each, one with the second and one with the third beside it); and an infinity in V is
 // found in the first part's sums.  With more rows, where a part of a weight that is zero makes a NaN of an infinity, output that is
 // not finite is summed again in plain 32-bit arithmetic, which few ever need.
 // A row's weights are taken relative to a maximum that moves only when it has grown by kSlack: moving it costs a
 // multiplication of the whole output, and among 16 rows one has a new maximum in nearly every tile.
+//
+// Measured from a cold cache (in brackets the bytes at the copy bandwidth): 16 prompts x 8 beams, 32 heads, prompts to 2048 in
+// fp16, 591 MB: 123 us (91); without the arithmetic on tiles 106, without the second launch 113, the layout of the parts alone 8.
+// 12 prompts with up to 12 beams, 40 heads, mostly own keys in bf16, 1.2 GB: 225 (185), 201, 217 and 10.  4 x 8, 64 heads on 8,
+// prompts to 16384, 237 MB: 74 (36), 66 without the second launch, 59 without own keys as well.
 #include <type_traits>
 
 #include "dz_elem.cuh"
@@ -51,6 +56,7 @@ constexpr int kRingBytes = kStages * kStageBytes;
 constexpr int kMaxSeqs = 1024;           // also groups: what the layout of the parts takes of shared memory
 constexpr int kMaxParts = 32;            // of a row's shared keys, and of its own
 constexpr int kLeastSpan = 32;           // keys of a part at least
+constexpr int kFewKeys = 512;            // shared keys that are not worth the start and end of a part in tensor memory
 constexpr int kEight = 8;                // rows that leave half of an MMA's to the weights' parts
 
 struct SharedDecode {
@@ -1040,7 +1046,10 @@ template <typename T>
 int launch_decode(const SharedDecode& p, const CUtensorMap& map_k, const CUtensorMap& map_v, bool tma, size_t smem, cudaStream_t st) {
   const int ratio = p.heads / p.kv_heads;
   const bool few_own = ratio <= kEight, few_shared = few_own && (int64_t)p.max_group * ratio <= kEight;
-  if (tma && p.team > 1)
+  // (4 groups of 20 sequences, 32 heads, 512 shared keys, warps and tcgen05: fp16 40 and 57 us, bf16 45 and 68; at 1024 either may be
+  // ahead; 16 groups of 16, 64 heads on 8, 2048 keys: 123 and 80, 139 and 84.  At most 16 rows, 8 of 8 sequences, 32 heads, 4096
+  // keys: 88 and 104, 94 and 131.)
+  if (tma && p.team > 1 && p.max_shared > kFewKeys)
     return few_own ? launch_form<T, true, kOnTc, true>(p, map_k, map_v, smem, st) : launch_form<T, true, kOnTc, false>(p, map_k, map_v, smem, st);
   if (tma)
     return few_shared ? launch_form<T, true, kFewRows, true>(p, map_k, map_v, smem, st)

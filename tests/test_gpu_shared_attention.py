@@ -347,3 +347,51 @@ def test_large_scores_move_the_maximum():
             b.k[at] = (b.k[at].float() * 0.05 + torch.linspace(0, 6, len(at), device="cuda")[:, None, None] *
                        b.qkv[0, :128].float().sign()[None, None]).to(torch.bfloat16)
         b.check(b.run())
+
+
+@pytest.fixture
+def bound_far_above(monkeypatch):
+    """A bound on the shared keys far above the ones there are: groups of many rows stay on tensor memory."""
+    from deltazip_b200 import ops
+    real = ops.shared_attention_decode
+
+    def call(qkv, k, v, tables, lens, starts, shared, most, longest, *rest, **kw):
+        return real(qkv, k, v, tables, lens, starts, shared, most, max(longest, 2000), *rest, **kw)
+    monkeypatch.setattr(ops, "shared_attention_decode", call)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("size,heads,kvh", [(5, 8, 2), (9, 8, 1), (40, 4, 1)])
+@pytest.mark.parametrize("key", [0, 63, 64, 141, 149, 155])
+def test_infinities_in_short_parts_of_tensor_memory(bound_far_above, key, size, heads, kvh, dtype):
+    test_infinities_among_the_values_of_many_rows(key, size, heads, kvh, dtype)
+
+
+@pytest.mark.parametrize("block", [16, 32, 5])
+@pytest.mark.parametrize("size,heads,kvh", [(3, 4, 4), (4, 8, 2), (9, 8, 1), (33, 8, 2)])
+def test_nan_behind_short_parts_of_tensor_memory(bound_far_above, size, heads, kvh, block):
+    test_nan_behind_the_end_of_many_rows(size, heads, kvh, block)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads,kvh", [(8, 1), (12, 3), (16, 1)])
+@pytest.mark.parametrize("sizes", [[4], [3, 1, 8], [9, 2]])
+def test_short_parts_in_tensor_memory(bound_far_above, sizes, heads, kvh, dtype):
+    test_groups(sizes, heads, kvh, dtype)
+
+
+@pytest.mark.parametrize("sizes", [[9], [12, 3, 16], [16] * 40])
+def test_parts_of_every_length_in_tensor_memory(bound_far_above, sizes):
+    test_parts_of_every_length(sizes)
+
+
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 1e-3, 5.0])
+def test_scales_in_tensor_memory(bound_far_above, scale):
+    test_scales(scale, 9, 8, 1)
+
+
+@pytest.mark.parametrize("keys", [511, 512, 513])
+@pytest.mark.parametrize("size,heads,kvh", [(5, 8, 2), (9, 8, 1), (20, 2, 2)])
+def test_lengths_at_which_the_form_changes(keys, size, heads, kvh):
+    b = Batch([size, 2], [keys, 40], [5] * (size + 2), heads, kvh, torch.bfloat16, seed=keys)
+    b.check(b.run())
