@@ -14,7 +14,7 @@
 //           one after the other.
 // Bound: the logits' bytes, and for a few rows the two launches.  A piece costs a CTA as much again as its loads: three
 // instructions of an exponential an element, the maxima, and what it takes to collect and rank what reaches the floor, which
-// is why the floor rises with every piece (73 us before, 57 with it, as both were then).  Measured from a cold cache: 284 rows of
+// is why the floor rises with every piece (74 us before, 58 with it, as both were then).  Measured from a cold cache: 284 rows of
 // 131072 tokens in bf16, groups of up to 16, k = 32 (74 MB, 11.4 us at the copy bandwidth): 47 us, 37 of them before the second
 // launch; 128 rows of 32000 floats, k = 16: 21 us; 4 rows, k = 8: 14.  (The first with every thread naming its best, k times, as
 // the only way: 180 us in a row of calls, where it takes 42.)

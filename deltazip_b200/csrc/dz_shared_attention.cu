@@ -1046,8 +1046,8 @@ template <typename T>
 int launch_decode(const SharedDecode& p, const CUtensorMap& map_k, const CUtensorMap& map_v, bool tma, size_t smem, cudaStream_t st) {
   const int ratio = p.heads / p.kv_heads;
   const bool few_own = ratio <= kEight, few_shared = few_own && (int64_t)p.max_group * ratio <= kEight;
-  // (4 groups of 20 sequences, 32 heads, 512 shared keys, warps and tcgen05: fp16 40 and 57 us, bf16 45 and 68; at 1024 either may be
-  // ahead; 16 groups of 16, 64 heads on 8, 2048 keys: 123 and 80, 139 and 84.  At most 16 rows, 8 of 8 sequences, 32 heads, 4096
+  // (4 groups of 20 sequences, 32 heads, 512 shared keys, warps and tcgen05: fp16 42 and 60 us, bf16 48 and 67; at 1024 either may be
+  // ahead; 16 groups of 16, 64 heads on 8, 2048 keys: 124 and 81, 140 and 85.  At most 16 rows, 8 of 8 sequences, 32 heads, 4096
   // keys: 88 and 104, 94 and 131.)
   if (tma && p.team > 1 && p.max_shared > kFewKeys)
     return few_own ? launch_form<T, true, kOnTc, true>(p, map_k, map_v, smem, st) : launch_form<T, true, kOnTc, false>(p, map_k, map_v, smem, st);
