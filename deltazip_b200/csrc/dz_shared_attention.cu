@@ -34,6 +34,10 @@
 // bf16: two of half the first part each, one with the second and one with the third beside it); and an infinity in V is
 // found in the first part's sums.  With more rows, where a part of a weight that is zero makes a NaN of an infinity, output that is
 // not finite is summed again in plain 32-bit arithmetic, which few ever need.
+// An accumulator of the tensor cores cuts off what it cannot hold instead of rounding it (measured: up to 2^-22 of the sum an
+// addition, all with one sign), so a long sum falls short by its length.  No more than 384 products go into one: 2048 keys on
+// warps, 4096 on tcgen05 in two accumulators; then the output joins what the rounds before have left, in 32-bit arithmetic.
+// (Over 65536 keys of one part: off by at most 2^-16.5 of the sum of absolute products, without rounds by up to 2^-11.2.)
 // A row's weights are taken relative to a maximum that moves only when it has grown by kSlack: moving it costs a
 // multiplication of the whole output, and among 16 rows one has a new maximum in nearly every tile.
 //
@@ -57,6 +61,7 @@ constexpr int kMaxSeqs = 1024;           // also groups: what the layout of the 
 constexpr int kMaxParts = 32;            // of a row's shared keys, and of its own
 constexpr int kLeastSpan = 32;           // keys of a part at least
 constexpr int kFewKeys = 512;            // shared keys that are not worth the start and end of a part in tensor memory
+constexpr int kSumTiles = 128;           // tiles that are summed before the output leaves the registers
 constexpr int kEight = 8;                // rows that leave half of an MMA's to the weights' parts
 
 struct SharedDecode {
@@ -92,9 +97,9 @@ __device__ __forceinline__ int chunk_at(int r, int c) { return (c >> 3) * (kHalf
 __device__ __forceinline__ int quarter(int c, int t) { return (c >> 1) * 8 + 2 * t + (c & 1); }
 
 // Scores are kept times log2 e, and weights are 2^(score - maximum + kLift), at most 2^(kLift + kSlack).  They enter the
-// products with V as sums of 16-bit numbers: two of fp16 hold 22 bits, as many as the exponential's own error leaves (of weights
-// above 2^-12 of the largest; below, what is lost is at most 2^-35 of it, which no sum with the largest can hold), bf16
-// takes three for its 24.
+// products with V as sums of 16-bit numbers: two of fp16 hold 22 bits of a weight, as many as the exponential's own error leaves
+// (of weights above 2^-12 of the largest; below, what is lost is at most 2^-35 of it, which no sum with the largest can hold),
+// bf16 takes three for a weight's 24.
 constexpr int kSlack = 4;
 template <typename T> constexpr int kLift = 0;
 template <> constexpr int kLift<__half> = 11;
@@ -325,8 +330,14 @@ __device__ __forceinline__ void run_parts(const SharedDecode& p, const Layout& a
   const float scale = p.scale * kLog2e;
   constexpr int kHalves = kFew ? 1 : 2;                        // rows gq, and gq + 8
   constexpr bool kDoubled = kFew && kParts<T> == 3;            // weights of half the size, whose first parts count twice
-  for (; unit < units; unit += teams) {
-    const Part part = part_of(unit);
+  int round = 0;                         // of the part: kSumTiles are summed, and join what the rounds before have left
+  while (unit < units) {
+    Part part = part_of(unit);
+    const int end = part.t1;
+    part.t0 += round * (kSumTiles * kTile);
+    part.t_lo = max(part.t_lo, part.t0);
+    part.t1 = min(end, part.t0 + kSumTiles * kTile);
+    part.tiles = (part.t1 - part.t0 + kTile - 1) / kTile;
     const int mine = part.row0 + member * kRows;
     uint4 q[kHalves][4];                                       // absent rows are zero
 #pragma unroll
@@ -466,30 +477,52 @@ __device__ __forceinline__ void run_parts(const SharedDecode& p, const Layout& a
       }
     }
     bool finite = true;
+    float2 was[kHalves];
 #pragma unroll
     for (int h = 0; h < kHalves; ++h) {
       l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
       l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+      if (kDoubled) l[h] *= 2.f;
+      const int r = mine + gq + 8 * h, seq = part.seq0 + r / ratio;
+      was[h] = make_float2(-INFINITY, 0.f);
+      if (round > 0 && r < part.rows) was[h] = p.ml[((size_t)seq * p.heads + part.kvh * ratio + r % ratio) * p.parts + part.index];
+    }
+    __syncwarp();
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) {
       const int r = mine + gq + 8 * h, seq = part.seq0 + r / ratio;
       if (r < part.rows && (own || at.common[seq] > 0)) {      // (otherwise it reads all of its keys by itself)
         const size_t to = ((size_t)seq * p.heads + part.kvh * ratio + r % ratio) * p.parts + part.index;
         float* out = p.partial + to * kDim + 2 * t;
+        const float now = fmaxf(m[h], was[h].x), c = m[h] == now ? 1.f : exp2_of(m[h] - now);
+        const float before = was[h].x == -INFINITY ? 0.f : exp2_of(was[h].x - now);
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           float2 v = make_float2(o[j][2 * h], o[j][2 * h + 1]);
           if (kFew) {                                          // (an infinity is what the first parts make of it)
             if (isfinite(v.x)) v.x += o[j][2];
             if (isfinite(v.y)) v.y += o[j][3];
-          } else {
-            finite = finite && ((isfinite(v.x) && isfinite(v.y)) || !(l[h] == l[h]));       // (a sum that is NaN stays one)
           }
+          if (round > 0) {
+            const float2 w = *reinterpret_cast<const float2*>(out + j * 8);
+            v.x = v.x * c + w.x * before;
+            v.y = v.y * c + w.y * before;
+          }
+          if (!kFew) finite = finite && ((isfinite(v.x) && isfinite(v.y)) || !(l[h] == l[h]));       // (a sum that is NaN stays one)
           *reinterpret_cast<float2*>(out + j * 8) = v;
         }
-        if (t == 0) p.ml[to] = make_float2(m[h], kDoubled ? 2.f * l[h] : l[h]);
+        m[h] = now;
+        if (t == 0) p.ml[to] = make_float2(now, l[h] * c + was[h].y * before);
       }
+    }
+    if (part.t1 < end) {
+      ++round;
+      __syncwarp();
+      continue;
     }
     if (!kFew && __any_sync(0xffffffffu, !finite)) {
       __syncwarp();
+      part = part_of(unit);
       for (int i = 0; i < kRows; ++i) {
         const int r = mine + i, seq = part.seq0 + r / ratio;
         if (r >= part.rows || (!own && at.common[seq] == 0)) continue;
@@ -499,6 +532,8 @@ __device__ __forceinline__ void run_parts(const SharedDecode& p, const Layout& a
         *reinterpret_cast<float4*>(p.partial + to * kDim + lane * 4) = v;
       }
     }
+    round = 0;
+    unit += teams;
   }
   if (!kTma) cp_async_wait<0>();
   // the team's rings change hands
@@ -509,6 +544,7 @@ __device__ __forceinline__ void run_parts(const SharedDecode& p, const Layout& a
 // The parts of shared keys that fall to the CTA, on tcgen05.
 constexpr int kTcRows = 128, kTcKeys = 64, kTcStages = 5;
 constexpr int kTcSlabQ = kTcRows * 128, kTcSlab = kTcKeys * 128, kTcQ = 2 * kTcSlabQ, kTcStage = 4 * kTcSlab;
+constexpr int kTcSumTiles = 64;          // tiles that are summed before the output leaves tensor memory (32: 83 us for 77, see above)
 constexpr int kTcBuffer = 96, kTcOut = 2 * kTcBuffer;          // columns of tensor memory: scores and weights' parts, twice; two outputs
 static_assert(kTcQ + kTcStages * kTcStage <= kWarps * kRingBytes, "the rings' place holds it");
 struct TcBarriers {
@@ -560,7 +596,11 @@ __device__ __forceinline__ void run_rows_tc(const SharedDecode& p, const Layout&
   const uint32_t s_q = smem_addr(smem), s_kv = s_q + kTcQ;
   auto wait = [&](uint64_t& b, uint32_t parity) { mbar_wait(smem_addr(&b), parity, at.abort, p.status); };
   auto tiles_of = [](const Part& x) { return (x.t1 - x.t0 + kTcKeys - 1) / kTcKeys; };
-  uint32_t c = 0, n = 0;                                       // tiles and parts so far
+  auto tiles_at_a_time = [](int tiles) {                       // a part is summed in rounds of about as many tiles
+    const int rounds = (tiles + kTcSumTiles - 1) / kTcSumTiles;
+    return (tiles + rounds - 1) / rounds;
+  };
+  uint32_t c = 0, n = 0;                                       // tiles and rounds so far
   if (warp == 4 || warp == 5) {
     // ---- copies: K by one warp, V by the other ----
     const bool values = warp == 5;
@@ -625,27 +665,30 @@ __device__ __forceinline__ void run_rows_tc(const SharedDecode& p, const Layout&
         for (int k = 0; k < 4; ++k) warp_umma_ss(d, a + s * (kTcSlabQ >> 4) + 2 * k, b + s * (kTcSlab >> 4) + 2 * k, id_s, s + k > 0);
       warp_umma_commit(smem_addr(&bar.scores[c & 1]));
     };
-    for (int u = blockIdx.x; u < units; u += gridDim.x, ++n) {
-      const int tiles = tiles_of(shared_part(p, at, u, kTcRows));
-      wait(bar.queries, n & 1);
-      __syncwarp();
-      scores(c);
-      if (tiles > 1) scores(c + 1);
-      for (int j = 0; j < tiles; ++j, ++c) {
-        const uint32_t st = c % kTcStages, buffer = tmem + (c & 1) * kTcBuffer;
-        wait(bar.weights[c & 1], (c >> 1) & 1);
+    for (int u = blockIdx.x; u < units; u += gridDim.x) {
+      const int all = tiles_of(shared_part(p, at, u, kTcRows)), most = tiles_at_a_time(all);
+      for (int t0 = 0; t0 < all; t0 += most, ++n) {
+        const int tiles = min(most, all - t0);
+        wait(bar.queries, n & 1);
         __syncwarp();
-        tc_fence_after();
-        const uint32_t v = desc_lo_mn(s_kv + st * kTcStage + 2 * kTcSlab, kTcSlab);
+        scores(c);
+        if (tiles > 1) scores(c + 1);
+        for (int j = 0; j < tiles; ++j, ++c) {
+          const uint32_t st = c % kTcStages, buffer = tmem + (c & 1) * kTcBuffer;
+          wait(bar.weights[c & 1], (c >> 1) & 1);
+          __syncwarp();
+          tc_fence_after();
+          const uint32_t v = desc_lo_mn(s_kv + st * kTcStage + 2 * kTcSlab, kTcSlab);
 #pragma unroll
-        for (int k = 0; k < kTcKeys / 16; ++k)                 // 16 keys: 2048 bytes of V, 8 columns of a part
+          for (int k = 0; k < kTcKeys / 16; ++k)                 // 16 keys: 2048 bytes of V, 8 columns of a part
 #pragma unroll
-          for (int w = 0; w < kParts<T>; ++w)
-            warp_umma_ts(tmem + kTcOut + (j & 1) * kDim, buffer + w * 32 + k * 8, v + k * 128, id_o, j > 1 || k > 0 || w > 0);
-        warp_umma_commit(smem_addr(&bar.empty[st]));
-        warp_umma_commit(smem_addr(&bar.products[j & 1]));
-        if (j + 2 < tiles) scores(c + 2);                      // behind the product that reads these columns' weights
-        if (j + 1 == tiles) warp_umma_commit(smem_addr(&bar.outputs));
+            for (int w = 0; w < kParts<T>; ++w)
+              warp_umma_ts(tmem + kTcOut + (j & 1) * kDim, buffer + w * 32 + k * 8, v + k * 128, id_o, j > 1 || k > 0 || w > 0);
+          warp_umma_commit(smem_addr(&bar.empty[st]));
+          warp_umma_commit(smem_addr(&bar.products[j & 1]));
+          if (j + 2 < tiles) scores(c + 2);                      // behind the product that reads these columns' weights
+          if (j + 1 == tiles) warp_umma_commit(smem_addr(&bar.outputs));
+        }
       }
     }
   } else if (warp < 4 || warp >= 8) {
@@ -655,137 +698,161 @@ __device__ __forceinline__ void run_rows_tc(const SharedDecode& p, const Layout&
     const float scale = p.scale == 0.f ? 1.f : fabsf(p.scale) * kLog2e;
     const uint32_t lanes = (uint32_t)(w4 * 32) << 16, t_o = tmem + kTcOut + odd * kDim + lanes;
     uint32_t k = 0;                                            // tiles of this kind so far
-    for (int u = blockIdx.x; u < units; u += gridDim.x, ++n) {
+    for (int u = blockIdx.x; u < units; u += gridDim.x) {
       const Part part = shared_part(p, at, u, kTcRows);
-      const int row = part.row0 + r, tiles = tiles_of(part), seq = part.seq0 + row / ratio;
+      const int row = part.row0 + r, all = tiles_of(part), most = tiles_at_a_time(all), seq = part.seq0 + row / ratio;
       const bool there = row < part.rows, any = part.row0 + w4 * 32 < part.rows;         // the row; any of the warp's
-      if (!odd) {
-        const T* from = (const T*)p.q + (size_t)seq * p.q_stride + (size_t)(part.kvh * ratio + row % ratio) * kDim;
-        const uint32_t turn = p.scale < 0.f ? 0x80008000u : 0u;
+      const bool mine = there && at.common[min(seq, p.seqs - 1)] > 0;      // (otherwise it reads all of its keys by itself)
+      const size_t to = ((size_t)seq * p.heads + part.kvh * ratio + row % ratio) * p.parts + part.index;
+      float part_m = -INFINITY, part_l = 0.f;                  // of the rounds so far
+      bool finite = true;
+      for (int t0 = 0; t0 < all; t0 += most, ++n) {
+        const int tiles = min(most, all - t0);
+        if (!odd && t0 > 0) {
+          if (lane == 0) mbar_arrive(smem_addr(&bar.queries));   // (they stay; the output has been taken)
+        } else if (!odd) {
+          const T* from = (const T*)p.q + (size_t)seq * p.q_stride + (size_t)(part.kvh * ratio + row % ratio) * kDim;
+          const uint32_t turn = p.scale < 0.f ? 0x80008000u : 0u;
 #pragma unroll 4
-        for (int i = 0; i < 16; ++i) {
-          uint4 v = there && p.scale != 0.f ? *reinterpret_cast<const uint4*>(from + i * 8) : make_uint4(0, 0, 0, 0);
-          v = make_uint4(v.x ^ turn, v.y ^ turn, v.z ^ turn, v.w ^ turn);
-          sts128(s_q + (i >> 3) * kTcSlabQ + r * 128 + (((i ^ r) & 7) << 4), v);
+          for (int i = 0; i < 16; ++i) {
+            uint4 v = there && p.scale != 0.f ? *reinterpret_cast<const uint4*>(from + i * 8) : make_uint4(0, 0, 0, 0);
+            v = make_uint4(v.x ^ turn, v.y ^ turn, v.z ^ turn, v.w ^ turn);
+            sts128(s_q + (i >> 3) * kTcSlabQ + r * 128 + (((i ^ r) & 7) << 4), v);
+          }
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_addr(&bar.queries));
+        } else {
+          wait(bar.queries, n & 1);                              // the even tiles' warps are through with the round before
+          __syncwarp();
         }
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_addr(&bar.queries));
-      } else {
-        wait(bar.queries, n & 1);                              // the even tiles' warps are through with the part before
-        __syncwarp();
-      }
-      float m = -INFINITY, l = 0.f;
-      for (int j = odd; j < tiles; j += 2) {
-        const uint32_t tile = c + j, t_s = tmem + (tile & 1) * kTcBuffer + lanes;
-        wait(bar.scores[tile & 1], (tile >> 1) & 1);
+        float m = -INFINITY, l = 0.f;
+        for (int j = odd; j < tiles; j += 2) {
+          const uint32_t tile = c + j, t_s = tmem + (tile & 1) * kTcBuffer + lanes;
+          wait(bar.scores[tile & 1], (tile >> 1) & 1);
+          __syncwarp();
+          tc_fence_after();
+          if (any) {
+            float s[kTcKeys];
+            tmem_ld32(t_s, s);
+            tmem_ld32(t_s + 32, s + 32);
+            tmem_wait_ld();
+            const int valid = part.t1 - part.t0 - (t0 + j) * kTcKeys;
+            if (valid < kTcKeys) {
+#pragma unroll
+              for (int i = 0; i < kTcKeys; ++i) s[i] = i < valid ? s[i] : -INFINITY;
+            }
+            float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+            for (int i = 4; i < kTcKeys; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+            float f = 1.f;
+            if (top > m + kSlack) {
+              f = exp2_of(m - top);
+              m = top;
+              l *= f;
+            }
+            const float off = kLift<T> - (m == -INFINITY ? 0.f : m);
+            const unsigned long long mul = pair_of(scale, scale), add = pair_of(off, off);
+            unsigned long long sum[2] = {pair_of(0.f, 0.f), pair_of(0.f, 0.f)};
+#pragma unroll
+            for (int i = 0; i < kTcKeys; i += 32) {
+              uint32_t parts[3][16];
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                float a, b;
+                halves_of(fma_pair(pair_of(s[i + 2 * e], s[i + 2 * e + 1]), mul, add), a, b);
+                a = exp2_of(a);
+                b = exp2_of(b);
+                sum[e & 1] = add_pair(sum[e & 1], pair_of(a, b));
+                cut_weights<T>(a, b, parts[0][e], parts[1][e], parts[2][e]);
+              }
+#pragma unroll
+              for (int w = 0; w < kParts<T>; ++w) tmem_st16(t_s + w * 32 + i / 2, parts[w]);
+            }
+            float la, lb;
+            halves_of(add_pair(sum[0], sum[1]), la, lb);
+            l += la + lb;
+            if (j > 1 && __any_sync(0xffffffffu, f != 1.f)) {
+              wait(bar.products[odd], (k - 1) & 1);              // the output holds the products so far
+              __syncwarp();
+              tc_fence_after();
+              for (int i = 0; i < kDim; i += 32) {
+                float o[32];
+                tmem_ld32(t_o + i, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] *= f;
+                tmem_st16(t_o + i, reinterpret_cast<const uint32_t*>(o));
+                tmem_st16(t_o + i + 16, reinterpret_cast<const uint32_t*>(o + 16));
+              }
+            }
+            tmem_wait_st();
+          }
+          ++k;
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_addr(&bar.weights[tile & 1]));
+        }
+        c += tiles;
+        if (odd) {
+          bar.m[r] = m;
+          bar.l[r] = l;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_addr(&bar.odd));
+          continue;
+        }
+        // the even tiles' warps join both, and what the rounds before have left
+        wait(bar.odd, n & 1);
+        wait(bar.outputs, n & 1);
         __syncwarp();
         tc_fence_after();
         if (any) {
-          float s[kTcKeys];
-          tmem_ld32(t_s, s);
-          tmem_ld32(t_s + 32, s + 32);
-          tmem_wait_ld();
-          const int valid = part.t1 - part.t0 - j * kTcKeys;
-          if (valid < kTcKeys) {
+          const float m1 = bar.m[r], now = fmaxf(fmaxf(m, m1), part_m);
+          const float f0 = m == -INFINITY ? 0.f : exp2_of(m - now), f1 = m1 == -INFINITY ? 0.f : exp2_of(m1 - now);
+          const float before = part_m == -INFINITY ? 0.f : exp2_of(part_m - now);
+          part_m = now;
+          part_l = part_l * before + l * f0 + bar.l[r] * f1;
+          for (int i = 0; i < kDim; i += 32) {
+            float o[32], o1[32];
+            tmem_ld32(t_o + i, o);
+            if (tiles > 1) tmem_ld32(t_o + kDim + i, o1);
+            tmem_wait_ld();
+            if (mine) {
+              float4* out = reinterpret_cast<float4*>(p.partial + to * kDim + i);
 #pragma unroll
-            for (int i = 0; i < kTcKeys; ++i) s[i] = i < valid ? s[i] : -INFINITY;
-          }
-          float mx[4] = {s[0], s[1], s[2], s[3]};
+              for (int e = 0; e < 32; ++e) {
+                o[e] *= f0;
+                if (tiles > 1) o[e] += o1[e] * f1;
+              }
+              if (t0 > 0) {
 #pragma unroll
-          for (int i = 4; i < kTcKeys; ++i) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
-          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
-          float f = 1.f;
-          if (top > m + kSlack) {
-            f = exp2_of(m - top);
-            m = top;
-            l *= f;
-          }
-          const float off = kLift<T> - (m == -INFINITY ? 0.f : m);
-          const unsigned long long mul = pair_of(scale, scale), add = pair_of(off, off);
-          unsigned long long sum[2] = {pair_of(0.f, 0.f), pair_of(0.f, 0.f)};
+                for (int e = 0; e < 32; e += 4) {
+                  const float4 was = out[e / 4];
+                  o[e] += was.x * before;
+                  o[e + 1] += was.y * before;
+                  o[e + 2] += was.z * before;
+                  o[e + 3] += was.w * before;
+                }
+              }
 #pragma unroll
-          for (int i = 0; i < kTcKeys; i += 32) {
-            uint32_t parts[3][16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              float a, b;
-              halves_of(fma_pair(pair_of(s[i + 2 * e], s[i + 2 * e + 1]), mul, add), a, b);
-              a = exp2_of(a);
-              b = exp2_of(b);
-              sum[e & 1] = add_pair(sum[e & 1], pair_of(a, b));
-              cut_weights<T>(a, b, parts[0][e], parts[1][e], parts[2][e]);
-            }
-#pragma unroll
-            for (int w = 0; w < kParts<T>; ++w) tmem_st16(t_s + w * 32 + i / 2, parts[w]);
-          }
-          float la, lb;
-          halves_of(add_pair(sum[0], sum[1]), la, lb);
-          l += la + lb;
-          if (j > 1 && __any_sync(0xffffffffu, f != 1.f)) {
-            wait(bar.products[odd], (k - 1) & 1);              // the output holds the products so far
-            __syncwarp();
-            tc_fence_after();
-            for (int i = 0; i < kDim; i += 32) {
-              float o[32];
-              tmem_ld32(t_o + i, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] *= f;
-              tmem_st16(t_o + i, reinterpret_cast<const uint32_t*>(o));
-              tmem_st16(t_o + i + 16, reinterpret_cast<const uint32_t*>(o + 16));
+              for (int e = 0; e < 32; e += 4) {
+                finite = finite && isfinite(o[e]) && isfinite(o[e + 1]) && isfinite(o[e + 2]) && isfinite(o[e + 3]);
+                out[e / 4] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+              }
             }
           }
-          tmem_wait_st();
+          tc_fence_before();
         }
-        ++k;
-        tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_addr(&bar.weights[tile & 1]));
       }
-      c += tiles;
-      if (odd) {
-        bar.m[r] = m;
-        bar.l[r] = l;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_addr(&bar.odd));
-        continue;
-      }
-      // the even tiles' warps join both
-      wait(bar.odd, n & 1);
-      wait(bar.outputs, n & 1);
-      __syncwarp();
-      tc_fence_after();
-      if (!any) continue;
-      const float m1 = bar.m[r], both = fmaxf(m, m1);
-      const float f0 = m == -INFINITY ? 0.f : exp2_of(m - both), f1 = m1 == -INFINITY ? 0.f : exp2_of(m1 - both);
-      l = l * f0 + bar.l[r] * f1;
-      const bool mine = there && at.common[min(seq, p.seqs - 1)] > 0;      // (otherwise it reads all of its keys by itself)
-      const size_t to = ((size_t)seq * p.heads + part.kvh * ratio + row % ratio) * p.parts + part.index;
-      bool finite = true;
-      for (int i = 0; i < kDim; i += 32) {
-        float o[32], o1[32];
-        tmem_ld32(t_o + i, o);
-        if (tiles > 1) tmem_ld32(t_o + kDim + i, o1);
-        tmem_wait_ld();
-        if (mine) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            o[e] *= f0;
-            if (tiles > 1) o[e] += o1[e] * f1;
-            finite = finite && isfinite(o[e]);
-          }
-#pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            *reinterpret_cast<float4*>(p.partial + to * kDim + i + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-        }
-      }
-      if (mine) p.ml[to] = make_float2(both, l);
-      uint32_t again = __ballot_sync(0xffffffffu, !finite && l == l);      // (a sum that is NaN stays one)
+      if (odd || !any) continue;
+      if (mine) p.ml[to] = make_float2(part_m, part_l);
+      uint32_t again = __ballot_sync(0xffffffffu, !finite && part_l == part_l);      // (a sum that is NaN stays one)
       __syncwarp();
       for (; again; again &= again - 1) {
         const int from = __ffs(again) - 1;
-        const float4 v = sum_plainly<T>(p, part, __shfl_sync(0xffffffffu, row, from), __shfl_sync(0xffffffffu, both, from));
+        const float4 v = sum_plainly<T>(p, part, __shfl_sync(0xffffffffu, row, from), __shfl_sync(0xffffffffu, part_m, from));
         const unsigned long long place = __shfl_sync(0xffffffffu, (unsigned long long)to, from);
         *reinterpret_cast<float4*>(p.partial + place * kDim + lane * 4) = v;
       }

@@ -395,3 +395,33 @@ def test_scales_in_tensor_memory(bound_far_above, scale):
 def test_lengths_at_which_the_form_changes(keys, size, heads, kvh):
     b = Batch([size, 2], [keys, 40], [5] * (size + 2), heads, kvh, torch.bfloat16, seed=keys)
     b.check(b.run())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("groups,size,rep,kvh,own", [(37, 4, 8, 4, False), (222, 2, 8, 8, False), (222, 1, 1, 8, False), (222, 1, 1, 8, True)])
+def test_sums_over_long_spans(groups, size, rep, kvh, own, dtype):
+    """65536 keys in one part, in tensor memory, on warps with sixteen rows and on warps with few, whose output the last two
+    keys cancel, so that its own rounding is out of the way.  Allowed against the sum of absolute products: at most 384
+    products of 16 keys go into one accumulator (half of 4096 keys, or 2048, in three parts), an addition loses up to
+    2^-22 of a sum that grows evenly to half of the absolute sum -- 384 * 2^-22 / 4 = 2^-15.4 -- and all else, the scores of
+    the last two keys above all, stays below 2^-17: 2^-14.9 together.  (The losses have one sign: over all 65536 keys they
+    come to between 2^-13 and 2^-11.)"""
+    from deltazip_b200 import ops
+    n, seqs = 65536, groups * size
+    g = torch.Generator("cuda").manual_seed(groups + size)
+    q = torch.randn((kvh, 128), generator=g, device="cuda").to(dtype)
+    k = torch.randn((n, kvh, 128), generator=g, device="cuda").to(dtype)
+    v = (1 + torch.rand((n, kvh, 128), generator=g, device="cuda")).to(dtype)
+    k[-2:] = q                                     # weights of the size of all the others together
+    w = (torch.einsum("hd,nhd->hn", q.double(), k.double()) * SCALE).softmax(1)
+    for j in (n - 2, n - 1):                       # each takes away what the keys before it leave
+        v[j] = (-torch.einsum("hn,nhd->hd", w[:, :j], v[:j].double()) / w[:, j, None]).to(dtype)
+    heads = kvh * rep
+    qkv = torch.cat([q.repeat_interleave(rep, 0).reshape(-1), torch.zeros(2 * kvh * 128, device="cuda", dtype=dtype)])
+    shared = [0 if own else n] * groups
+    out = ops.shared_attention_decode(qkv.repeat(seqs, 1), k, v, i32([list(range(n // 16))]).repeat(seqs, 1), i32([n] * seqs),
+                                      i32(list(range(0, seqs + 1, size))), i32(shared), size, max(shared), heads, kvh, 16, SCALE)
+    assert torch.equal(out, out[:1].expand_as(out))
+    want, parts = torch.einsum("hn,nhd->hd", w, v.double()), torch.einsum("hn,nhd->hd", w, v.double().abs())
+    err = (out[0].view(kvh, rep, 128).double() - want[:, None]).abs() / parts[:, None]
+    assert float(err.max()) <= 2.0 ** -14.9, float(err.max())
