@@ -32,8 +32,9 @@
 // (Eight rows in this manner and in that of more, 8 groups of 8, 32 heads: 512 keys 41 and 45 us, 4096 keys 88 both.)
 // With up to eight rows the other eight of an MMA carry the other parts (fp16: one MMA with the first and the second part;
 // bf16: two of half the first part each, one with the second and one with the third beside it); and an infinity in V is
-// found in the first part's sums.  With more rows, where a part of a weight that is zero makes a NaN of an infinity, output that is
-// not finite is summed again in plain 32-bit arithmetic, which few ever need.
+// found in the first part's sums.  With more rows, where a part of a weight that is zero makes a NaN of an infinity, a part whose
+// output is not finite has its values looked through once, for all of a warp's rows, and those components set to what they
+// call for.
 // An accumulator of the tensor cores cuts off what it cannot hold instead of rounding it (measured: up to 2^-22 of the sum an
 // addition, all with one sign), so a long sum falls short by its length.  No more than 384 products go into one: 2048 keys on
 // warps, 4096 on tcgen05 in two accumulators; then the output joins what the rounds before have left, in 32-bit arithmetic.
@@ -185,27 +186,43 @@ __device__ __forceinline__ uint32_t cache_row(const SharedDecode& p, const int* 
   return min(page * p.block_size + (key - b * p.block_size), p.last_row);
 }
 
-// The output of one row over a part in plain arithmetic, a warp together: lane i has components 4 i ... 4 i + 3.
+// What is not finite in a part's values: three bits for each of the lane's components 4 lane ... 4 lane + 3 (NaN, +inf, -inf).
+// A warp together, once for all of its rows: a value takes as long as any other byte of the cache.
 template <typename T>
-__device__ __noinline__ float4 sum_plainly(const SharedDecode& p, Part part, int r, float m) {
-  const int lane = threadIdx.x & 31, ratio = p.heads / p.kv_heads;
-  auto four = [&](const T* from) {
-    const uint2 v = *reinterpret_cast<const uint2*>(from + lane * 4);
-    const float2 a = Cvt<T>::up(v.x), b = Cvt<T>::up(v.y);
-    return make_float4(a.x, a.y, b.x, b.y);
-  };
-  const float4 q = four((const T*)p.q + (size_t)(part.seq0 + r / ratio) * p.q_stride + (size_t)(part.kvh * ratio + r % ratio) * kDim);
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int key = part.t_lo; key < part.t1; ++key) {
-    const size_t at = ((size_t)cache_row(p, p.tables + (size_t)part.source * p.width, key) * p.kv_heads + part.kvh) * kDim;
-    const float4 k = four((const T*)p.k_cache + at), v = four((const T*)p.v_cache + at);
-    const float w = exp2_of(warp_sum(q.x * k.x + q.y * k.y + q.z * k.z + q.w * k.w) * (p.scale * kLog2e) - m + kLift<T>);
-    o.x += w * v.x;
-    o.y += w * v.y;
-    o.z += w * v.z;
-    o.w += w * v.w;
+__device__ __noinline__ uint32_t not_finite(const SharedDecode& p, Part part) {
+  const int lane = threadIdx.x & 31, *table = p.tables + (size_t)part.source * p.width;
+  uint32_t seen = 0;
+  for (int key0 = part.t_lo; key0 < part.t1; key0 += 32) {
+    const uint32_t row = cache_row(p, table, min(key0 + lane, part.t1 - 1));
+    const int n = min(32, part.t1 - key0);
+#pragma unroll 16
+    for (int i = 0; i < n; ++i) {
+      const size_t at = ((size_t)__shfl_sync(0xffffffffu, row, i) * p.kv_heads + part.kvh) * kDim + lane * 4;
+      const uint2 v = *reinterpret_cast<const uint2*>((const T*)p.v_cache + at);
+      const float2 a = Cvt<T>::up(v.x), b = Cvt<T>::up(v.y);
+      const float f[4] = {a.x, a.y, b.x, b.y};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (!isfinite(f[e])) seen |= (f[e] > 0.f ? 2u : f[e] < 0.f ? 4u : 1u) << 3 * e;
+    }
   }
-  return o;
+  return seen;
+}
+// What a component that is not finite becomes: an infinity among the values has a positive weight, so the output is that
+// infinity, and NaN where a value is NaN or there are both.  (Without any of them a sum has overflowed, and stays.)
+__device__ __forceinline__ float settled(float v, uint32_t seen) {
+  if (isfinite(v) || seen == 0) return v;
+  return seen == 2u ? INFINITY : seen == 4u ? -INFINITY : NAN;
+}
+// ... of a row's output over a part, a warp together.
+__device__ __forceinline__ void settle_row(float* out, uint32_t seen) {
+  float4* at = reinterpret_cast<float4*>(out) + (threadIdx.x & 31);
+  float4 v = *at;
+  v.x = settled(v.x, seen & 7);
+  v.y = settled(v.y, seen >> 3 & 7);
+  v.z = settled(v.z, seen >> 6 & 7);
+  v.w = settled(v.w, seen >> 9 & 7);
+  *at = v;
 }
 
 // Where the parts are, in shared memory.
@@ -508,7 +525,7 @@ __device__ __forceinline__ void run_parts(const SharedDecode& p, const Layout& a
             v.x = v.x * c + w.x * before;
             v.y = v.y * c + w.y * before;
           }
-          if (!kFew) finite = finite && ((isfinite(v.x) && isfinite(v.y)) || !(l[h] == l[h]));       // (a sum that is NaN stays one)
+          if (!kFew) finite = finite && isfinite(v.x) && isfinite(v.y);
           *reinterpret_cast<float2*>(out + j * 8) = v;
         }
         m[h] = now;
@@ -522,14 +539,12 @@ __device__ __forceinline__ void run_parts(const SharedDecode& p, const Layout& a
     }
     if (!kFew && __any_sync(0xffffffffu, !finite)) {
       __syncwarp();
-      part = part_of(unit);
+      const uint32_t seen = not_finite<T>(p, part_of(unit));
       for (int i = 0; i < kRows; ++i) {
         const int r = mine + i, seq = part.seq0 + r / ratio;
-        if (r >= part.rows || (!own && at.common[seq] == 0)) continue;
         const float mr = __shfl_sync(0xffffffffu, i < 8 ? m[0] : m[kHalves - 1], (i & 7) * 4);
-        const size_t to = ((size_t)seq * p.heads + part.kvh * ratio + r % ratio) * p.parts + part.index;
-        const float4 v = sum_plainly<T>(p, part, r, mr);
-        *reinterpret_cast<float4*>(p.partial + to * kDim + lane * 4) = v;
+        if (r >= part.rows || mr == -INFINITY || (!own && at.common[seq] == 0)) continue;        // (no weight is positive)
+        settle_row(p.partial + (((size_t)seq * p.heads + part.kvh * ratio + r % ratio) * p.parts + part.index) * kDim, seen);
       }
     }
     round = 0;
@@ -848,14 +863,11 @@ __device__ __forceinline__ void run_rows_tc(const SharedDecode& p, const Layout&
       }
       if (odd || !any) continue;
       if (mine) p.ml[to] = make_float2(part_m, part_l);
-      uint32_t again = __ballot_sync(0xffffffffu, !finite && part_l == part_l);      // (a sum that is NaN stays one)
+      uint32_t again = __ballot_sync(0xffffffffu, !finite && part_m > -INFINITY);
       __syncwarp();
-      for (; again; again &= again - 1) {
-        const int from = __ffs(again) - 1;
-        const float4 v = sum_plainly<T>(p, part, __shfl_sync(0xffffffffu, row, from), __shfl_sync(0xffffffffu, part_m, from));
-        const unsigned long long place = __shfl_sync(0xffffffffu, (unsigned long long)to, from);
-        *reinterpret_cast<float4*>(p.partial + place * kDim + lane * 4) = v;
-      }
+      const uint32_t seen = again ? not_finite<T>(p, part) : 0;
+      for (; again; again &= again - 1)
+        settle_row(p.partial + __shfl_sync(0xffffffffu, (unsigned long long)to, __ffs(again) - 1) * kDim, seen);
     }
   }
 }

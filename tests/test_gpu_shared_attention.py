@@ -425,3 +425,33 @@ def test_sums_over_long_spans(groups, size, rep, kvh, own, dtype):
     want, parts = torch.einsum("hn,nhd->hd", w, v.double()), torch.einsum("hn,nhd->hd", w, v.double().abs())
     err = (out[0].view(kvh, rep, 128).double() - want[:, None]).abs() / parts[:, None]
     assert float(err.max()) <= 2.0 ** -14.9, float(err.max())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("size,heads,kvh", [(8, 64, 8), (2, 64, 8)])
+def test_nan_and_infinities_in_a_long_prompt(size, heads, kvh, dtype):
+    """What is not finite in one prompt's values costs a look through them and not a sum a row: the other prompts' outputs keep
+    their bits, no wait runs out, and the call stays within 10 ms (a row summed by itself takes some 2 ms, of 32 a warp)."""
+    from deltazip_b200 import ops
+    b = Batch([size] * 4, [16384, 9000, 16000, 5000], [20] * (4 * size), heads, kvh, dtype, seed=size)
+    args = [b.qkv, b.k, b.v, i32(b.tables), i32(b.lens), i32(b.starts), i32(b.shared), size, 16384, heads, kvh, 16, SCALE]
+    clean, rep = ops.shared_attention_decode(*args), heads // kvh
+    for key, comp, value in ((3, 5, float("nan")), (7000, 9, float("inf")), (8999, 9, float("-inf")), (8000, 77, float("inf")),
+                             (17, 100, float("-inf"))):
+        for s in range(size, 2 * size):            # (page or copy: the same row for all, or one of each)
+            b.v[b.slot(s, key), 3, comp] = value
+    times = []
+    for _ in range(3):
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        start.record()
+        out = ops.shared_attention_decode(*args)
+        end.record()
+        end.synchronize()
+        times.append(start.elapsed_time(end))
+    assert ops.read_status() == 0
+    bad = torch.zeros_like(out, dtype=torch.bool).view(4 * size, kvh, rep, 128)
+    bad[size:2 * size, 3, :, [5, 9, 77, 100]] = True
+    assert torch.equal(out.view_as(bad)[~bad], clean.view_as(bad)[~bad])
+    got = out.view_as(bad)[size:2 * size, 3]
+    assert got[..., [5, 9]].isnan().all() and (got[..., 77] == float("inf")).all() and (got[..., 100] == float("-inf")).all()
+    assert min(times) <= 10, times
