@@ -31,10 +31,9 @@
 //            ldmatrix.
 // (Eight rows in this manner and in that of more, 8 groups of 8, 32 heads: 512 keys 41 and 45 us, 4096 keys 88 both.)
 // With up to eight rows the other eight of an MMA carry the other parts (fp16: one MMA with the first and the second part;
-// bf16: two of half the first part each, one with the second and one with the third beside it); and an infinity in V is
-// found in the first part's sums.  With more rows, where a part of a weight that is zero makes a NaN of an infinity, a part whose
-// output is not finite has its values looked through once, for all of a warp's rows, and those components set to what they
-// call for.
+// bf16: two of half the first part each, one with the second and one with the third beside it).  Where a part of a weight is
+// zero it makes a NaN of an infinity among the values.  So a row that comes out not finite has its values looked through as
+// it is joined, and those components set to what they call for.
 // An accumulator of the tensor cores cuts off what it cannot hold instead of rounding it (measured: up to 2^-22 of the sum an
 // addition, all with one sign), so a long sum falls short by its length.  No more than 384 products go into one: 2048 keys on
 // warps, 4096 on tcgen05 in two accumulators; then the output joins what the rounds before have left, in 32-bit arithmetic.
@@ -184,45 +183,6 @@ __device__ __forceinline__ uint32_t cache_row(const SharedDecode& p, const int* 
   const uint32_t b = (uint32_t)((uint64_t)(uint32_t)key * p.block_magic >> p.block_shift);
   const uint32_t page = min((uint32_t)table[b], p.last_page);
   return min(page * p.block_size + (key - b * p.block_size), p.last_row);
-}
-
-// What is not finite in a part's values: three bits for each of the lane's components 4 lane ... 4 lane + 3 (NaN, +inf, -inf).
-// A warp together, once for all of its rows: a value takes as long as any other byte of the cache.
-template <typename T>
-__device__ __noinline__ uint32_t not_finite(const SharedDecode& p, Part part) {
-  const int lane = threadIdx.x & 31, *table = p.tables + (size_t)part.source * p.width;
-  uint32_t seen = 0;
-  for (int key0 = part.t_lo; key0 < part.t1; key0 += 32) {
-    const uint32_t row = cache_row(p, table, min(key0 + lane, part.t1 - 1));
-    const int n = min(32, part.t1 - key0);
-#pragma unroll 16
-    for (int i = 0; i < n; ++i) {
-      const size_t at = ((size_t)__shfl_sync(0xffffffffu, row, i) * p.kv_heads + part.kvh) * kDim + lane * 4;
-      const uint2 v = *reinterpret_cast<const uint2*>((const T*)p.v_cache + at);
-      const float2 a = Cvt<T>::up(v.x), b = Cvt<T>::up(v.y);
-      const float f[4] = {a.x, a.y, b.x, b.y};
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (!isfinite(f[e])) seen |= (f[e] > 0.f ? 2u : f[e] < 0.f ? 4u : 1u) << 3 * e;
-    }
-  }
-  return seen;
-}
-// What a component that is not finite becomes: an infinity among the values has a positive weight, so the output is that
-// infinity, and NaN where a value is NaN or there are both.  (Without any of them a sum has overflowed, and stays.)
-__device__ __forceinline__ float settled(float v, uint32_t seen) {
-  if (isfinite(v) || seen == 0) return v;
-  return seen == 2u ? INFINITY : seen == 4u ? -INFINITY : NAN;
-}
-// ... of a row's output over a part, a warp together.
-__device__ __forceinline__ void settle_row(float* out, uint32_t seen) {
-  float4* at = reinterpret_cast<float4*>(out) + (threadIdx.x & 31);
-  float4 v = *at;
-  v.x = settled(v.x, seen & 7);
-  v.y = settled(v.y, seen >> 3 & 7);
-  v.z = settled(v.z, seen >> 6 & 7);
-  v.w = settled(v.w, seen >> 9 & 7);
-  *at = v;
 }
 
 // Where the parts are, in shared memory.
@@ -493,7 +453,6 @@ __device__ __forceinline__ void run_parts(const SharedDecode& p, const Layout& a
         }
       }
     }
-    bool finite = true;
     float2 was[kHalves];
 #pragma unroll
     for (int h = 0; h < kHalves; ++h) {
@@ -516,16 +475,15 @@ __device__ __forceinline__ void run_parts(const SharedDecode& p, const Layout& a
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           float2 v = make_float2(o[j][2 * h], o[j][2 * h + 1]);
-          if (kFew) {                                          // (an infinity is what the first parts make of it)
-            if (isfinite(v.x)) v.x += o[j][2];
-            if (isfinite(v.y)) v.y += o[j][3];
+          if (kFew) {
+            v.x += o[j][2];
+            v.y += o[j][3];
           }
           if (round > 0) {
             const float2 w = *reinterpret_cast<const float2*>(out + j * 8);
             v.x = v.x * c + w.x * before;
             v.y = v.y * c + w.y * before;
           }
-          if (!kFew) finite = finite && isfinite(v.x) && isfinite(v.y);
           *reinterpret_cast<float2*>(out + j * 8) = v;
         }
         m[h] = now;
@@ -536,16 +494,6 @@ __device__ __forceinline__ void run_parts(const SharedDecode& p, const Layout& a
       ++round;
       __syncwarp();
       continue;
-    }
-    if (!kFew && __any_sync(0xffffffffu, !finite)) {
-      __syncwarp();
-      const uint32_t seen = not_finite<T>(p, part_of(unit));
-      for (int i = 0; i < kRows; ++i) {
-        const int r = mine + i, seq = part.seq0 + r / ratio;
-        const float mr = __shfl_sync(0xffffffffu, i < 8 ? m[0] : m[kHalves - 1], (i & 7) * 4);
-        if (r >= part.rows || mr == -INFINITY || (!own && at.common[seq] == 0)) continue;        // (no weight is positive)
-        settle_row(p.partial + (((size_t)seq * p.heads + part.kvh * ratio + r % ratio) * p.parts + part.index) * kDim, seen);
-      }
     }
     round = 0;
     unit += teams;
@@ -720,7 +668,6 @@ __device__ __forceinline__ void run_rows_tc(const SharedDecode& p, const Layout&
       const bool mine = there && at.common[min(seq, p.seqs - 1)] > 0;      // (otherwise it reads all of its keys by itself)
       const size_t to = ((size_t)seq * p.heads + part.kvh * ratio + row % ratio) * p.parts + part.index;
       float part_m = -INFINITY, part_l = 0.f;                  // of the rounds so far
-      bool finite = true;
       for (int t0 = 0; t0 < all; t0 += most, ++n) {
         const int tiles = min(most, all - t0);
         if (!odd && t0 > 0) {
@@ -852,7 +799,6 @@ __device__ __forceinline__ void run_rows_tc(const SharedDecode& p, const Layout&
               }
 #pragma unroll
               for (int e = 0; e < 32; e += 4) {
-                finite = finite && isfinite(o[e]) && isfinite(o[e + 1]) && isfinite(o[e + 2]) && isfinite(o[e + 3]);
                 out[e / 4] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
               }
             }
@@ -863,11 +809,6 @@ __device__ __forceinline__ void run_rows_tc(const SharedDecode& p, const Layout&
       }
       if (odd || !any) continue;
       if (mine) p.ml[to] = make_float2(part_m, part_l);
-      uint32_t again = __ballot_sync(0xffffffffu, !finite && part_m > -INFINITY);
-      __syncwarp();
-      const uint32_t seen = again ? not_finite<T>(p, part) : 0;
-      for (; again; again &= again - 1)
-        settle_row(p.partial + __shfl_sync(0xffffffffu, (unsigned long long)to, __ffs(again) - 1) * kDim, seen);
     }
   }
 }
@@ -1056,6 +997,29 @@ shared_decode_kernel(const __grid_constant__ SharedDecode p, const __grid_consta
   run_parts<T, kTma, kFewOwn>(p, at, &map_k, &map_v, true, smem, used);
 }
 
+// What is not finite among the first `length` values of a sequence: three bits (NaN, +inf, -inf) for each of the lane's
+// components 4 lane ... 4 lane + 3.  A warp together; 16 cache rows on their way at a time.
+template <typename T>
+__device__ __noinline__ uint32_t not_finite(const SharedDecode& p, int seq, int kvh, int length) {
+  const int lane = threadIdx.x & 31, *table = p.tables + (size_t)seq * p.width;
+  uint32_t seen = 0;
+  for (int key0 = 0; key0 < length; key0 += 32) {
+    const uint32_t row = cache_row(p, table, min(key0 + lane, length - 1));
+    const int n = min(32, length - key0);
+#pragma unroll 16
+    for (int i = 0; i < n; ++i) {
+      const size_t at = ((size_t)__shfl_sync(0xffffffffu, row, i) * p.kv_heads + kvh) * kDim + lane * 4;
+      const uint2 v = *reinterpret_cast<const uint2*>((const T*)p.v_cache + at);
+      const float2 a = Cvt<T>::up(v.x), b = Cvt<T>::up(v.y);
+      const float f[4] = {a.x, a.y, b.x, b.y};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (!isfinite(f[e])) seen |= (f[e] > 0.f ? 2u : f[e] < 0.f ? 4u : 1u) << 3 * e;
+    }
+  }
+  return seen;
+}
+
 // A warp per row: the parts' outputs by the weight of their maxima.
 template <typename T>
 __global__ void __launch_bounds__(256) shared_join_kernel(SharedDecode p) {
@@ -1088,6 +1052,18 @@ __global__ void __launch_bounds__(256) shared_join_kernel(SharedDecode p) {
     }
   }
   sum = warp_sum(sum);
+  // An infinity among the values has a positive weight, so the output is that infinity, and NaN where a value is NaN or there are
+  // both.  (Where a part of a weight, or a part's weight here, is zero its product is NaN.  A key with a score of -inf counts like
+  // any other.  Without such a value a sum has overflowed, and stays.)
+  const bool finite = isfinite(a[0]) && isfinite(a[1]) && isfinite(a[2]) && isfinite(a[3]);
+  if (sum > 0.f && __any_sync(0xffffffffu, !finite)) {
+    const uint32_t seen = not_finite<T>(p, seq, row % p.heads / (p.heads / p.kv_heads), length);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t mine = seen >> 3 * e & 7;
+      if (mine) a[e] = mine == 2 ? INFINITY : mine == 4 ? -INFINITY : NAN;
+    }
+  }
   uint2 v = make_uint2(Cvt<T>::down(a[0] / sum, a[1] / sum), Cvt<T>::down(a[2] / sum, a[3] / sum));
   if (parts == 0) v = make_uint2(0, 0);
   *reinterpret_cast<uint2*>((T*)p.out + (size_t)row * kDim + lane * 4) = v;

@@ -455,3 +455,30 @@ def test_nan_and_infinities_in_a_long_prompt(size, heads, kvh, dtype):
     got = out.view_as(bad)[size:2 * size, 3]
     assert got[..., [5, 9]].isnan().all() and (got[..., 77] == float("inf")).all() and (got[..., 100] == float("-inf")).all()
     assert min(times) <= 10, times
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("size,heads,kvh", [(1, 1, 1), (8, 2, 2), (2, 8, 2), (9, 2, 2), (40, 2, 2)])
+@pytest.mark.parametrize("below", [30, 45, 60, 100])
+def test_infinities_far_below_the_maximum(below, size, heads, kvh, dtype):
+    """A value of a key whose score is so far below the largest that its weight rounds to zero, in the part of that one and
+    in another: what the definition gives does not depend on how many rows there are."""
+    b = Batch([size, 1], [600, 40], [20] * (size + 1), heads, kvh, dtype, seed=below)
+    b.qkv[:] = b.qkv[0].sign()
+    b.k *= 0.02
+    u = b.qkv[0, :128]
+    b.qkv[:, :heads * 128] = u.repeat(heads)
+    for s in range(size):
+        b.k[b.slot(s, 100)] = (u.float() * (below / (128 * SCALE))).to(dtype)
+        b.v[b.slot(s, 101), :, 7], b.v[b.slot(s, 599), :, 12], b.v[b.slot(s, 610), :, 20] = float("inf"), float("-inf"), float("inf")
+        b.v[b.slot(s, 90), :, 33], b.v[b.slot(s, 580), :, 33], b.v[b.slot(s, 615), :, 50] = float("inf"), float("-inf"), float("nan")
+    for longest in (600, 2000):
+        out = b.run(longest=longest).view(size + 1, heads, 128)
+        for s in range(size):
+            want = b.want(s).view(heads, 128)
+            assert want[:, [7, 12, 20]].isinf().all() and want[:, [33, 50]].isnan().all()
+            odd = ~want.isfinite()
+            assert int(odd.sum()) == 5 * heads and torch.equal(out[s].isfinite(), ~odd)
+            assert torch.equal(torch.where(out[s].isnan(), 1., out[s].double())[odd], torch.where(want.isnan(), 1., want)[odd])
+            err = (out[s].double()[~odd] - want[~odd]).norm() / want[~odd].norm()
+            assert err <= TOL[dtype]
