@@ -45,7 +45,7 @@ class _Beams:
     def __init__(self, number: int, root: Sequence):
         self.number, self.root, self.first_id = number, root, root.seq_id
         self.seqs, self.tokens, self.scores = [root], [[]], [0.0]
-        self.common = 0                 # leading cache blocks that all hypotheses hold
+        self.common = 0                 # leading cache blocks that all hypotheses hold and have filled
         self.ended: List[Hypothesis] = []
 
     def end(self, tokens: List[int], score: float, keep: int, penalty: float) -> None:
@@ -61,10 +61,10 @@ class _Beams:
         length = max_new if penalty > 0 else len(self.tokens[0]) + 1
         return self.scores[0] / length ** penalty <= self.ended[-1].score
 
-    def shared_blocks(self) -> int:
-        blocks = [s.blocks for s in self.seqs]
-        most = min(map(len, blocks))
-        while self.common < most and len({b[self.common] for b in blocks}) == 1:
+    def shared_blocks(self, block_size: int) -> int:
+        """Leading blocks that all hypotheses hold and none will write to again (later ones go on from these)."""
+        blocks, full = [s.blocks for s in self.seqs], min(s.length for s in self.seqs) // block_size
+        while self.common < full and len({b[self.common] for b in blocks}) == 1:
             self.common += 1
         return self.common
 
@@ -468,8 +468,7 @@ class DecodeEngine:
         self._rebuild(tokens)
         active.sort(key=lambda g: self._sort_key(g.seqs[0]))
         self.groups = ([len(g.seqs) for g in active],
-                       [min(g.shared_blocks() * self.block_size, min(s.length for s in g.seqs)) if self.cache.window is None else 0
-                        for g in active])
+                       [g.shared_blocks(self.block_size) * self.block_size if self.cache.window is None else 0 for g in active])
 
     def _select(self, groups: List[_Beams], hidden: torch.Tensor, keep: int, beams: int, max_new: int, stop_id: Optional[int],
                 penalty: float, active: List[_Beams], out: List[List[Hypothesis]]) -> None:

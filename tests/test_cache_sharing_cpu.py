@@ -206,3 +206,32 @@ def test_states_fork_with_their_sequences():
     c.consistent([a, b, d])
     c.close(b)
     assert c.state.free == [b.state_slot] or b.state_slot == -1
+
+
+def test_what_one_hypothesis_holds_is_not_shared_when_it_forks():
+    """A prompt left with one hypothesis, whose written, partly written and reserved blocks are all its own, forks inside a
+    block: only the full blocks both hold count as shared, and both read what they wrote."""
+    from deltazip_b200.engine import _Beams
+    c = Cache(32)
+    root = seq(0)
+    c.open(root, 26)
+    g = _Beams(0, root)
+    for t in range(5):
+        c.write(root, t)
+    assert g.shared_blocks(4) == 1
+    c.write(root, 5)
+    child = seq(1, root.length)
+    c.fork([(root, child)])
+    g.seqs = [root, child]
+    assert c.own([(s, 1) for s in g.seqs])
+    assert g.shared_blocks(4) == 1
+    for step in range(10):
+        for i, s in enumerate(g.seqs):
+            c.write(s, 100 * (i + 1) + step)
+        c.own([(s, 1) for s in g.seqs])
+        shared = g.shared_blocks(4)
+        assert shared * 4 <= 6 and all(s.blocks[:shared] == root.blocks[:shared] for s in g.seqs)
+    assert [c.read(s)[6:] for s in g.seqs] == [[100 * (i + 1) + step for step in range(10)] for i in range(2)]
+    c.close(child)
+    g.seqs = [root]
+    assert g.shared_blocks(4) == 4                    # 16 tokens are written, and blocks behind them reserved

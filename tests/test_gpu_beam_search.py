@@ -232,3 +232,31 @@ def test_command_line(tmp_path, capsys):
     assert [[h["tokens"] for h in f] for f in got] == [[h.tokens for h in f] for f in want]
     assert main(args) == 0
     assert [json.loads(line) for line in capsys.readouterr().out.splitlines()] == eng.generate([[1, 2, 3], [9, 8, 7, 6]], 5)
+
+
+@pytest.mark.parametrize("length", [5, 21, 32])
+def test_one_hypothesis_that_forks_later(length, monkeypatch):
+    """A step that leaves one candidate, and steps behind it that leave many: what the one hypothesis held is not taken for
+    shared where its heirs write."""
+    eng = small_llama(kv_blocks=600)
+    prompts = prompts_of([length, length + 9], 384, length)
+    plain, calls = eng.model.beam_logits, []
+
+    def masked(hidden):
+        logits = plain(hidden)
+        calls.append(len(calls))
+        if calls[-1] in (0, 1):
+            logits = torch.full_like(logits, -float("inf"))
+            logits[:, 5 + calls[-1]] = 0
+        return logits
+    monkeypatch.setattr(eng.model, "beam_logits", masked)
+    got = eng.beam_search(prompts, 9, 4)
+    monkeypatch.setattr(eng.model, "beam_logits", plain)
+    through(eng)
+    for p, found in zip(prompts, got):
+        assert len(found) == 4 and len({tuple(h.tokens) for h in found}) == 4
+        for h in found:
+            assert h.tokens[:2] == [5, 6]
+            lp = log_probs(eng, [p + h.tokens[:-1]], len(p))[0]
+            alone = sum(float(lp[i, t]) for i, t in enumerate(h.tokens) if i > 1) / len(h.tokens)
+            assert abs(alone - h.score) <= 0.02, (alone, h.score)
