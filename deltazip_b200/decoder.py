@@ -28,6 +28,7 @@ class LayeredDecoder(nn.Module):
     """A subclass sets `layers` (DecoderLayers), calls `plan_cache` and adds its own tensors in
     `top_weights`."""
     supports_portions = True            # a prompt may be continued from the cache and state
+    whole_vocabulary = True             # logits are those of all tokens
 
     def __init__(self, cfg, device, seed: int, dtype: torch.dtype):
         super().__init__()

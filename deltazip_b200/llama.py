@@ -205,9 +205,14 @@ class LlamaForCausalLM(nn.Module):
         """fp32 logits over this rank's vocabulary rows (sampler math, not the hot path)."""
         return hidden_last.float() @ self.lm_head.float().t()
 
+    @property
+    def whole_vocabulary(self) -> bool:
+        """Whether this rank's logits are those of all tokens, as a beam search needs them."""
+        return self.lm_head.shape[0] == self.cfg.vocab_size
+
     def beam_logits(self, hidden: torch.Tensor) -> torch.Tensor:
         """What a beam search selects from: 32-bit sums of the 16-bit operands' products, over the whole vocabulary."""
-        if self.lm_head.shape[0] != self.cfg.vocab_size:
+        if not self.whole_vocabulary:
             raise ValueError("a beam search needs the whole vocabulary on one rank")
         return ops.matmul_f32(hidden, self.lm_head)
 

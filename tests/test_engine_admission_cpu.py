@@ -94,3 +94,17 @@ def test_overlapped_admission_starts_the_swap_in_and_admits_when_it_has_landed()
         eng.retire(s)
     assert eng.admit_overlapped(waiting, ready=lambda d: d in landed) == []
     assert eng.manager.log[-2:] == [("evict", 1), ("prefetch", 2)] and eng.swap_ins == 2
+
+
+def test_a_part_of_the_vocabulary_is_refused_before_a_prompt_runs():
+    import pytest
+    from deltazip_b200.llama import LlamaConfig, LlamaForCausalLM
+    cfg = LlamaConfig(hidden_size=256, intermediate_size=256, num_hidden_layers=0, num_attention_heads=2, num_key_value_heads=2,
+                      vocab_size=256)
+    eng = make_engine(2, [])
+    eng.manager, eng.model = None, LlamaForCausalLM(cfg, device="cpu")
+    assert eng.model.whole_vocabulary
+    eng.model.lm_head = torch.nn.Parameter(eng.model.lm_head[:128], requires_grad=False)
+    with pytest.raises(ValueError, match="whole vocabulary"):
+        eng.beam_search([[1, 2, 3]], 4, 2)
+    assert not eng.running and len(eng.cache.free) == 64
