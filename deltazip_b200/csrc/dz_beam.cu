@@ -34,14 +34,14 @@ constexpr int kRoom = 640;               // logits that are ranked by counting
 constexpr float kToLog2 = 1.4426950408889634f;                 // as a float, which is what the exponents are taken with
 constexpr double kLn2 = 0.6931471805599453;
 
-// Unsigned numbers in the order of the floats (no NaN comes here); 0 is below all of them.
+// Unsigned numbers in the order of the floats (no NaN comes here), -0 becoming the 0 that it equals; 0 is below all of them.
 __device__ __forceinline__ uint32_t ordered(float v) {
-  const uint32_t b = __float_as_uint(v);
+  const uint32_t b = __float_as_uint(v + 0.f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float unordered(uint32_t u) { return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u); }
 __device__ __forceinline__ uint64_t ordered(double v) {
-  const uint64_t b = (uint64_t)__double_as_longlong(v);
+  const uint64_t b = (uint64_t)__double_as_longlong(v + 0.);
   return b >> 63 ? ~b : b | (1ull << 63);
 }
 __device__ __forceinline__ double unordered(uint64_t u) {

@@ -178,3 +178,25 @@ def test_refusals():
             ops.beam_select(*args, 4)
     with pytest.raises(DeltaZipError):
         ops.beam_select(logits[:, :0], scores, starts, 4)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("vocab,k", [(2, 2), (40, 8), (5000, 24), (20000, 100)])
+def test_zeros_of_both_signs_are_equal(vocab, k, dtype):
+    """Logits multiplied by a mask: zeros of both signs among the best, at the k-th place and in all places; the lower token
+    comes first whatever its sign."""
+    from deltazip_b200 import ops
+    g = torch.Generator("cuda").manual_seed(vocab)
+    signs = torch.where(torch.rand((6, vocab), generator=g, device="cuda") < 0.5, -1., 1.)
+    logits = (torch.zeros((6, vocab), device="cuda") * signs).to(dtype)
+    logits[0, :vocab // 2], logits[0, vocab // 2:] = -0., 0.
+    logits[3:] = torch.where(torch.rand((3, vocab), generator=g, device="cuda") < 0.7, logits[3:].float(), -signs[3:].abs() * 2).to(dtype)
+    logits[4, vocab // 3] = 1
+    assert bool((logits.signbit() & (logits == 0)).any())
+    scores = torch.tensor([-1.5, -1.5, -0., 0., -1., -1.], device="cuda")
+    for starts in ([0, 1, 3, 6], [0, 6]):
+        check(ops.beam_select(logits, scores, i32(starts), k), reference(logits, scores, starts, k))
+    logits[:] = -1                                 # one token of a row has the whole probability: scores of both signs of zero
+    logits[:, 1] = INF
+    got = ops.beam_select(logits, torch.tensor([-0., 0., -0., 0., -0., 0.], device="cuda"), i32([0, 6]), 6)
+    assert got.rows.tolist() == [list(range(6))] and got.tokens.tolist() == [[1] * 6] and not got.scores.any()
