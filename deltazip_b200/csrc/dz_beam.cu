@@ -208,9 +208,11 @@ __global__ void __launch_bounds__(kThreads, 4) beam_rows_kernel(BeamRows p) {
       for (int j = 0; j < E; ++j) sum += exp2_of(fmaf(x[j], kToLog2, -new_ref));
       if (!(sum < INFINITY) || fabsf(new_ref) == INFINITY) {   // NaN, an infinity or very large logits among them
         sum = 0.f;
-#pragma unroll
-        for (int j = 0; j < E; ++j) sum += x[j] == new_top ? 1.f : x[j] < new_top ? exp2_of((x[j] - new_top) * kToLog2) : 0.f;
-        if (new_top == -INFINITY) sum = 0.f;
+#pragma unroll 1
+        for (int j = 0; j < (new_top > -INFINITY ? E : 0); ++j) {
+          const float v = Cvt<T>::one(ring[place(j)]);
+          if (v == v) sum += fabsf(new_ref) < INFINITY ? exp2_of(fmaf(v, kToLog2, -new_ref)) : v == new_top ? 1.f : exp2_of((v - new_top) * kToLog2);
+        }
       }
       if (new_top != top) total *= weight_of(top, ref, new_top, new_ref);
       total += sum;

@@ -200,3 +200,18 @@ def test_zeros_of_both_signs_are_equal(vocab, k, dtype):
     logits[:, 1] = INF
     got = ops.beam_select(logits, torch.tensor([-0., 0., -0., 0., -0., 0.], device="cuda"), i32([0, 6]), 6)
     assert got.rows.tolist() == [list(range(6))] and got.tokens.tolist() == [[1] * 6] and not got.scores.any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("offset", [-3000., 1000., 50000.])
+def test_nan_among_large_logits(offset, dtype):
+    """A NaN among the logits of some threads, of all, and of all but the first: the others' sum is as exact as without it."""
+    from deltazip_b200 import ops
+    vocab = 20000
+    logits, scores = inputs(6, vocab, torch.float32, 7)
+    logits = (logits + offset).to(dtype)
+    every = torch.arange(vocab, device="cuda")
+    for row, nan in enumerate((every % 997 == 3, every % 3 == 1, every > 0, every % 8 == 7, every < vocab - 40)):
+        logits[row, nan] = float("nan")
+    starts = [0, 1, 2, 3, 4, 5, 6]
+    check(ops.beam_select(logits, scores, i32(starts), 12), reference(logits, scores, starts, 12))
