@@ -215,3 +215,31 @@ def test_nan_among_large_logits(offset, dtype):
         logits[row, nan] = float("nan")
     starts = [0, 1, 2, 3, 4, 5, 6]
     check(ops.beam_select(logits, scores, i32(starts), 12), reference(logits, scores, starts, 12))
+
+
+@pytest.mark.parametrize("rows,vocab,dtype", [(3, 2 ** 30, torch.bfloat16), (9, 2 ** 28 + 3, torch.float32)])
+def test_offsets_beyond_32_bits(rows, vocab, dtype):
+    """The largest vocabulary, and rows that begin behind 2^32 bytes."""
+    from deltazip_b200 import ops
+    g = torch.Generator("cuda").manual_seed(rows)
+    logits = torch.empty((rows, vocab), dtype=dtype, device="cuda")
+    for row in logits:
+        row.normal_(0, 1, generator=g)
+    for row in range(rows):                        # the best in places of their own
+        logits[row, [vocab - 1 - row, 7, vocab // 2 + row]] = torch.tensor([30. - row, 29.5 - row, 31. - row], device="cuda").to(dtype)
+    scores = -torch.arange(rows, device="cuda").float()
+    got = ops.beam_select(logits, scores, i32([0, rows - 1, rows]), 6)
+    for group, (a, b) in enumerate(((0, rows - 1), (rows - 1, rows))):
+        want = []
+        for row in range(a, b):
+            z, lse = logits[row], 0.
+            for part in z.split(2 ** 27):
+                lse += float(part.double().exp().sum())
+            top = z.topk(8)
+            lse = float(torch.log(torch.tensor(lse, dtype=torch.float64)))
+            want += [(float(scores[row]) + float(x) - lse, row, int(t)) for x, t in zip(*top)]
+        want.sort(key=lambda c: (-c[0], c[1], c[2]))
+        assert got.rows[group, :3].tolist() == [r for _, r, _ in want[:3]]
+        assert got.tokens[group, :3].tolist() == [t for _, _, t in want[:3]]
+        for s, (w, _, _) in zip(got.scores[group, :3].tolist(), want):
+            assert abs(s - w) <= 55 * 2.0 ** -24 + abs(w) * 2.0 ** -24

@@ -179,3 +179,20 @@ def test_refusals():
                          ([torch.zeros((), device="cuda")], 1), ([pool, pool], 4), ([pool[:8], pool[4:12]], 4)):
         with pytest.raises(ValueError):
             ops.PagePools(tensors, per)
+
+
+def test_offsets_beyond_32_bits():
+    """Pages behind 2^33 bytes of a pool, in the form that reads all pairs first and in the one that does not."""
+    from deltazip_b200 import ops
+    pages, size = 140000, 64 * 1024
+    pool = torch.empty((pages, size), dtype=torch.uint8, device="cuda")
+    last = [pages - 1 - i for i in range(6)]
+    for i, p in enumerate(last):
+        pool[p] = i + 1
+    handle = ops.PagePools([pool], 1)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    ops.copy_pages(handle, ints(last[:2] + [5]), ints(last[2:4] + [6]))
+    assert [int(pool[p].float().mean()) for p in last] == [1, 2, 1, 2, 5, 6]
+    ops.copy_pages(handle, ints([last[0], last[5]]), ints([last[5], last[0]]))
+    assert [int(pool[p].float().mean()) for p in last] == [6, 2, 1, 2, 5, 1]
+    assert all(bool((pool[p] == pool[p, 0]).all()) for p in last)

@@ -482,3 +482,50 @@ def test_infinities_far_below_the_maximum(below, size, heads, kvh, dtype):
             assert torch.equal(torch.where(out[s].isnan(), 1., out[s].double())[odd], torch.where(want.isnan(), 1., want)[odd])
             err = (out[s].double()[~odd] - want[~odd]).norm() / want[~odd].norm()
             assert err <= TOL[dtype]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rise", [0., 40.])
+@pytest.mark.parametrize("groups,size,rep,kvh,block", [(37, 5, 8, 4, 16), (111, 5, 8, 4, 24), (222, 3, 8, 4, 24), (222, 2, 5, 8, 16), (222, 1, 3, 8, 9),
+                                                       (222, 1, 1, 8, 16)])
+def test_parts_of_several_rounds(groups, size, rep, kvh, block, rise, dtype):
+    """Parts that are summed in several rounds, the last one short, in every form: tensor memory, teams of four and of two
+    warps, a warp of sixteen and of eight rows, with and without whole tiles a page; the maximum the same or rising."""
+    from deltazip_b200 import ops
+    n, fresh, heads = 9001, 37, kvh * rep
+    g = torch.Generator("cuda").manual_seed(groups + rep)
+    pages = -(-(n + fresh) // block)
+    u = torch.randn(128, generator=g, device="cuda").sign()
+    q = torch.randn((size, heads, 128), generator=g, device="cuda") * 0.5 + u
+    k = torch.randn((pages * block, kvh, 128), generator=g, device="cuda")
+    k += (torch.linspace(0, rise, pages * block, device="cuda") / (128 * SCALE))[:, None, None] * u
+    v = torch.randn((pages * block, kvh, 128), generator=g, device="cuda").to(dtype)
+    q, k = q.to(dtype), k.to(dtype)
+    qkv = torch.cat([q.reshape(size, -1), torch.zeros((size, 2 * kvh * 128), device="cuda", dtype=dtype)], 1).repeat(groups, 1)
+    lens = [n + fresh * (s % 2) for s in range(size)]
+    for shared in (n, 0):                          # with its group, and each by itself
+        out = ops.shared_attention_decode(qkv, k, v, i32([list(range(pages))]).repeat(groups * size, 1), i32(lens * groups),
+                                          i32(list(range(0, groups * size + 1, size))), i32([shared] * groups), size, shared, heads, kvh,
+                                          block, SCALE).view(groups, size, heads, 128)
+        assert torch.equal(out, out[:1].expand_as(out))
+        for s, length in enumerate(lens):
+            w = (torch.einsum("hrd,nhd->hrn", q[s].view(kvh, rep, 128).double(), k[:length].double()) * SCALE).softmax(-1)
+            want = torch.einsum("hrn,nhd->hrd", w, v[:length].double()).reshape(heads, 128)
+            err = (out[0, s].double() - want).norm() / want.norm()
+            assert err <= TOL[dtype], (shared, s, float(err))
+
+
+@pytest.mark.parametrize("size,heads,kvh,block", [(1, 8, 8, 16), (3, 32, 8, 16), (6, 32, 8, 16), (6, 32, 8, 40)])
+def test_offsets_beyond_32_bits(size, heads, kvh, block):
+    """A cache of 2^33 bytes and more, sequences in its last pages."""
+    from deltazip_b200 import ops
+    b = Batch([size, 2], [700, 100], [30] * (size + 2), heads, kvh, torch.float16, block=block, seed=block)
+    have = b.k.shape[0] // block
+    total = 2 ** 33 // (kvh * 256 * block) + have
+    k, v = (torch.empty((total * block, kvh, 128), dtype=torch.float16, device="cuda") for _ in range(2))
+    k[-have * block:], v[-have * block:] = b.k, b.v
+    want = b.run()
+    tables = [[p + total - have for p in row] for row in b.tables]
+    got = ops.shared_attention_decode(b.qkv, k, v, i32(tables), i32(b.lens), i32(b.starts), i32(b.shared), size, 700, heads, kvh,
+                                      block, SCALE)
+    assert torch.equal(got, want)
