@@ -47,17 +47,12 @@ __device__ __forceinline__ uint64_t ordered(double v) {
 __device__ __forceinline__ double unordered(uint64_t u) {
   return __longlong_as_double((long long)(u >> 63 ? u & ~(1ull << 63) : ~u));
 }
-__device__ __forceinline__ float exp2_of(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 // The weight of a sum whose largest logit is `top`, taken relative to 2^ref, ref being top log2 e, where the largest of all
 // are `all` and `all_ref`.  (Logits too large for a ref are further apart than any exponential reaches.)
 __device__ __forceinline__ float weight_of(float top, float ref, float all, float all_ref) {
   if (fabsf(ref) == INFINITY || fabsf(all_ref) == INFINITY) return top == all ? 1.f : 0.f;
-  return exp2_of(ref - all_ref);
+  return ex2(ref - all_ref);
 }
 
 // What is selected by: the larger value (0: none), then the lower place.
@@ -205,13 +200,13 @@ __global__ void __launch_bounds__(kThreads, 4) beam_rows_kernel(BeamRows p) {
       const float new_top = fmaxf(top, mine), new_ref = new_top * kToLog2;
       float sum = 0.f;
 #pragma unroll
-      for (int j = 0; j < E; ++j) sum += exp2_of(fmaf(x[j], kToLog2, -new_ref));
+      for (int j = 0; j < E; ++j) sum += ex2(fmaf(x[j], kToLog2, -new_ref));
       if (!(sum < INFINITY) || fabsf(new_ref) == INFINITY) {   // NaN, an infinity or very large logits among them
         sum = 0.f;
 #pragma unroll 1
         for (int j = 0; j < (new_top > -INFINITY ? E : 0); ++j) {
           const float v = Cvt<T>::one(ring[place(j)]);
-          if (v == v) sum += fabsf(new_ref) < INFINITY ? exp2_of(fmaf(v, kToLog2, -new_ref)) : v == new_top ? 1.f : exp2_of((v - new_top) * kToLog2);
+          if (v == v) sum += fabsf(new_ref) < INFINITY ? ex2(fmaf(v, kToLog2, -new_ref)) : v == new_top ? 1.f : ex2((v - new_top) * kToLog2);
         }
       }
       if (new_top != top) total *= weight_of(top, ref, new_top, new_ref);

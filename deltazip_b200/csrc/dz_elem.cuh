@@ -145,6 +145,11 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t& hi, uint3
 }
 
 constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float ex2(float x) {              // two units off at most; what is below 2^-126 is zero
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 // -- launches --------------------------------------------------------------------------------------
 template <typename K, typename... Args>

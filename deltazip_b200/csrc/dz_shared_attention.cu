@@ -115,12 +115,6 @@ __device__ __forceinline__ void split_weights(float a, float b, float times, uin
   else mid = Cvt<T>::down(a, b);
 }
 
-__device__ __forceinline__ float exp2_of(float x) {            // (what is below 2^-126 is zero)
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 __device__ __forceinline__ int length_of(const SharedDecode& p, int seq) { return min(max(p.lens[seq], 0), p.width * p.block_size); }
 
 // The last of `n` entries that starts at or before x.
@@ -406,7 +400,7 @@ __device__ __forceinline__ void run_parts(const SharedDecode& p, const Layout& a
         if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
           for (int h = 0; h < kHalves; ++h) {
-            const float mn = fmaxf(m[h], mx[h]), c = mn == m[h] ? 1.f : exp2_of(m[h] - mn);
+            const float mn = fmaxf(m[h], mx[h]), c = mn == m[h] ? 1.f : ex2(m[h] - mn);
             m[h] = mn;
             l[h] *= c;
 #pragma unroll
@@ -421,7 +415,7 @@ __device__ __forceinline__ void run_parts(const SharedDecode& p, const Layout& a
           const float off = (m[h] == -INFINITY ? 0.f : m[h]) - (kLift<T> - kDoubled);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const float w0 = exp2_of(x[i][h][0] - off), w1 = exp2_of(x[i][h][1] - off);
+            const float w0 = ex2(x[i][h][0] - off), w1 = ex2(x[i][h][1] - off);
             l[h] += w0 + w1;
             if constexpr (kFew) {
               split_weights<T>(w0, w1, kDoubled ? 2.f : 1.f, a[0][2 * i], a[0][2 * i + 1], a[1][2 * i + 1]);
@@ -470,8 +464,8 @@ __device__ __forceinline__ void run_parts(const SharedDecode& p, const Layout& a
       if (r < part.rows && (own || at.common[seq] > 0)) {      // (otherwise it reads all of its keys by itself)
         const size_t to = ((size_t)seq * p.heads + part.kvh * ratio + r % ratio) * p.parts + part.index;
         float* out = p.partial + to * kDim + 2 * t;
-        const float now = fmaxf(m[h], was[h].x), c = m[h] == now ? 1.f : exp2_of(m[h] - now);
-        const float before = was[h].x == -INFINITY ? 0.f : exp2_of(was[h].x - now);
+        const float now = fmaxf(m[h], was[h].x), c = m[h] == now ? 1.f : ex2(m[h] - now);
+        const float before = was[h].x == -INFINITY ? 0.f : ex2(was[h].x - now);
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           float2 v = make_float2(o[j][2 * h], o[j][2 * h + 1]);
@@ -515,23 +509,6 @@ struct TcBarriers {
   float m[kTcRows], l[kTcRows];                                // of the odd tiles
 };
 
-// Pairs of 32-bit operations in one instruction.
-__device__ __forceinline__ unsigned long long pair_of(float a, float b) {
-  unsigned long long v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
-  return v;
-}
-__device__ __forceinline__ void halves_of(unsigned long long v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ unsigned long long fma_pair(unsigned long long a, unsigned long long b, unsigned long long c) {
-  unsigned long long d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ unsigned long long add_pair(unsigned long long a, unsigned long long b) {
-  unsigned long long d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 // Two weights in their parts.  bf16: the first part is the upper half of the float as it stands, the second that of what it
 // leaves (which is exact), the third the rest, rounded.
 template <typename T>
@@ -540,7 +517,7 @@ __device__ __forceinline__ void cut_weights(float a, float b, uint32_t& hi, uint
     auto cut = [](float& a, float& b, uint32_t& part) {
       const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
       part = __byte_perm(ua, ub, 0x7632);
-      halves_of(fma_pair(pair_of(__uint_as_float(ua & 0xffff0000u), __uint_as_float(ub & 0xffff0000u)), pair_of(-1.f, -1.f), pair_of(a, b)), a, b);
+      fma2(Pair(__uint_as_float(ua & 0xffff0000u), __uint_as_float(ub & 0xffff0000u)), Pair(-1.f, -1.f), Pair(a, b)).get(a, b);
     };
     cut(a, b, hi);
     cut(a, b, mid);
@@ -710,30 +687,30 @@ __device__ __forceinline__ void run_rows_tc(const SharedDecode& p, const Layout&
             const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
             float f = 1.f;
             if (top > m + kSlack) {
-              f = exp2_of(m - top);
+              f = ex2(m - top);
               m = top;
               l *= f;
             }
             const float off = kLift<T> - (m == -INFINITY ? 0.f : m);
-            const unsigned long long mul = pair_of(scale, scale), add = pair_of(off, off);
-            unsigned long long sum[2] = {pair_of(0.f, 0.f), pair_of(0.f, 0.f)};
+            const Pair mul(scale, scale), add(off, off);
+            Pair sum[2] = {Pair(0.f, 0.f), Pair(0.f, 0.f)};
 #pragma unroll
             for (int i = 0; i < kTcKeys; i += 32) {
               uint32_t parts[3][16];
 #pragma unroll
               for (int e = 0; e < 16; ++e) {
                 float a, b;
-                halves_of(fma_pair(pair_of(s[i + 2 * e], s[i + 2 * e + 1]), mul, add), a, b);
-                a = exp2_of(a);
-                b = exp2_of(b);
-                sum[e & 1] = add_pair(sum[e & 1], pair_of(a, b));
+                fma2(Pair(s[i + 2 * e], s[i + 2 * e + 1]), mul, add).get(a, b);
+                a = ex2(a);
+                b = ex2(b);
+                sum[e & 1] = add2(sum[e & 1], Pair(a, b));
                 cut_weights<T>(a, b, parts[0][e], parts[1][e], parts[2][e]);
               }
 #pragma unroll
               for (int w = 0; w < kParts<T>; ++w) tmem_st16(t_s + w * 32 + i / 2, parts[w]);
             }
             float la, lb;
-            halves_of(add_pair(sum[0], sum[1]), la, lb);
+            add2(sum[0], sum[1]).get(la, lb);
             l += la + lb;
             if (j > 1 && __any_sync(0xffffffffu, f != 1.f)) {
               wait(bar.products[odd], (k - 1) & 1);              // the output holds the products so far
@@ -771,8 +748,8 @@ __device__ __forceinline__ void run_rows_tc(const SharedDecode& p, const Layout&
         tc_fence_after();
         if (any) {
           const float m1 = bar.m[r], now = fmaxf(fmaxf(m, m1), part_m);
-          const float f0 = m == -INFINITY ? 0.f : exp2_of(m - now), f1 = m1 == -INFINITY ? 0.f : exp2_of(m1 - now);
-          const float before = part_m == -INFINITY ? 0.f : exp2_of(part_m - now);
+          const float f0 = m == -INFINITY ? 0.f : ex2(m - now), f1 = m1 == -INFINITY ? 0.f : ex2(m1 - now);
+          const float before = part_m == -INFINITY ? 0.f : ex2(part_m - now);
           part_m = now;
           part_l = part_l * before + l * f0 + bar.l[r] * f1;
           for (int i = 0; i < kDim; i += 32) {
@@ -1038,7 +1015,7 @@ __global__ void __launch_bounds__(256) shared_join_kernel(SharedDecode p) {
   mm = warp_max(mm);
   for (int i0 = 0; i0 < parts; i0 += 32) {
     const float2 w = i0 + lane < parts ? ml[i0 + lane] : make_float2(-INFINITY, 0.f);
-    const float c = w.x == -INFINITY ? 0.f : exp2_of(w.x - mm);
+    const float c = w.x == -INFINITY ? 0.f : ex2(w.x - mm);
     sum += w.y * c;
     const int n = min(32, parts - i0);
 #pragma unroll 8

@@ -35,28 +35,6 @@ constexpr int kBiasTc = 4096;
 constexpr int kBiasPad = kTileM + kTileKeys - 2;        // distances from -kBiasPad up are in the table
 constexpr float kMaxGrowth = 8.f;
 
-// Pairs of 32-bit operations in one instruction.
-struct Pair {
-  unsigned long long v;
-  __device__ __forceinline__ Pair() {}
-  __device__ __forceinline__ Pair(float a, float b) {
-    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
-  }
-  __device__ __forceinline__ void get(float& a, float& b) const {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-  }
-};
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
-  Pair d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return d;
-}
-__device__ __forceinline__ Pair add2(Pair a, Pair b) {
-  Pair d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
-  return d;
-}
-
 // Two weights as hi + lo pairs.  bf16: hi is the upper half of the float as it stands, lo the rounded rest.
 template <typename T> __device__ __forceinline__ void split_weights(float a, float b, uint32_t& hi, uint32_t& lo) {
   if constexpr (std::is_same<T, __nv_bfloat16>::value) {
