@@ -12,12 +12,14 @@
 //   groups  a CTA joins its rows' maxima and sums, takes the entries of its spans' lists into registers, searches for a score
 //           that k to about 2 k of them reach, and ranks those by counting -- or, where too many are equal, takes the best
 //           one after the other.
-// Bound: the logits' bytes, and for a few rows the two launches.  A piece costs a CTA as much again as its loads: three
-// instructions of an exponential an element, the maxima, and what it takes to collect and rank what reaches the floor, which
-// is why the floor rises with every piece (74 us before, 58 with it, as both were then).  Measured from a cold cache: 284 rows of
-// 131072 tokens in bf16, groups of up to 16, k = 32 (74 MB, 11.4 us at the copy bandwidth): 47 us, 37 of them before the second
-// launch; 128 rows of 32000 floats, k = 16: 21 us; 4 rows, k = 8: 14.  (The first with every thread naming its best, k times, as
-// the only way: 180 us in a row of calls, where it takes 42.)
+// Bound: the logits' bytes, and for a few rows the two launches.  It is far from the bytes: a piece is a chain of barriers for its
+// CTA -- maxima, collecting, ranking, cutting -- and a floor that rises with every piece keeps what is ranked short (74 us
+// before, 58 with it, as both were then).  Measured from a cold cache: 284 rows of 131072 tokens in bf16, groups of up to 16,
+// k = 32 (74 MB, 11.4 us at the copy bandwidth): 48 us, of which the profiler gives the second launch 13; in the first, issue
+// slots are busy 67 % of the time that an SM has work, the special function unit 26 % and DRAM 25 %, and spans of nine and of
+// seven pieces leave some SMs idle.  128 rows of 32000 floats, k = 16: 24 us; 4 rows, k = 8: 15 to 17.  Not measured: masks
+// that leave fewer than k logits above -inf, where every piece goes the way of naming the best k times.
+// (The first with that as the only way: 180 us in a row of calls, where it takes 42.)
 // Sums are 32-bit within a thread's piece (at most 32 terms) and 64-bit beyond, and so are the scores that rows are compared by:
 // beams come close to one another, and which is ahead is not to hang on a rounding.
 #include "dz_elem.cuh"

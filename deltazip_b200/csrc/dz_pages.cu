@@ -12,7 +12,7 @@
 // A CTA of 256 threads keeps eight units a thread in flight, two CTAs an SM: 64 KB of reads, then as many writes.  More of
 // either were slower (1500 pages of 32 KB in 16 pools, 1.57 GB moved: two CTAs 267 us, three 286, four 318, six with half
 // the units 360): reads and writes of the same DRAM want to come in long runs.  At 6511 GB/s: 241 us.  Measured further: 96
-// forks inside pages, 200 MB: 31 us (31); 64 states in a new order, 541 MB: 94 to 103 us (83).
+// forks inside pages, 200 MB: 31 us (31); 64 states in a new order, 541 MB: 102 to 105 us (83).
 #include "dz_elem.cuh"
 
 namespace dz {

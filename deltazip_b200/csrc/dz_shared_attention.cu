@@ -42,9 +42,9 @@
 // multiplication of the whole output, and among 16 rows one has a new maximum in nearly every tile.
 //
 // Measured from a cold cache (in brackets the bytes at the copy bandwidth): 16 prompts x 8 beams, 32 heads, prompts to 2048 in
-// fp16, 591 MB: 123 us (91); without the arithmetic on tiles 106, without the second launch 113, the layout of the parts alone 8.
-// 12 prompts with up to 12 beams, 40 heads, mostly own keys in bf16, 1.2 GB: 225 (185), 201, 217 and 10.  4 x 8, 64 heads on 8,
-// prompts to 16384, 237 MB: 74 (36), 66 without the second launch, 59 without own keys as well.
+// fp16, 591 MB: 123 us (91).  12 prompts with up to 12 beams, 40 heads, mostly own keys in bf16, 1.2 GB: 225 (185).  4 x 8,
+// 64 heads on 8, prompts to 16384, 237 MB: 76 (36): 64 rows are two warps of softmax a tile, so two of four schedulers.  The second
+// launch is 10 to 13 of these by the profiler.
 #include <type_traits>
 
 #include "dz_elem.cuh"
@@ -975,23 +975,29 @@ shared_decode_kernel(const __grid_constant__ SharedDecode p, const __grid_consta
 }
 
 // What is not finite among the first `length` values of a sequence: three bits (NaN, +inf, -inf) for each of the lane's
-// components 4 lane ... 4 lane + 3.  A warp together; 16 cache rows on their way at a time.
+// components 4 lane ... 4 lane + 3.  A warp together; eight cache rows on their way at a time (more take the registers that keep
+// joining rows in flight: 4 to 6 us of every call).
 template <typename T>
 __device__ __noinline__ uint32_t not_finite(const SharedDecode& p, int seq, int kvh, int length) {
   const int lane = threadIdx.x & 31, *table = p.tables + (size_t)seq * p.width;
   uint32_t seen = 0;
   for (int key0 = 0; key0 < length; key0 += 32) {
-    const uint32_t row = cache_row(p, table, min(key0 + lane, length - 1));
-    const int n = min(32, length - key0);
-#pragma unroll 16
-    for (int i = 0; i < n; ++i) {
-      const size_t at = ((size_t)__shfl_sync(0xffffffffu, row, i) * p.kv_heads + kvh) * kDim + lane * 4;
-      const uint2 v = *reinterpret_cast<const uint2*>((const T*)p.v_cache + at);
-      const float2 a = Cvt<T>::up(v.x), b = Cvt<T>::up(v.y);
-      const float f[4] = {a.x, a.y, b.x, b.y};
+    const uint32_t row = cache_row(p, table, min(key0 + lane, length - 1));       // (the last again past the end)
+#pragma unroll 1
+    for (int i = 0; i < 32; i += 8) {
+      uint2 v[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (!isfinite(f[e])) seen |= (f[e] > 0.f ? 2u : f[e] < 0.f ? 4u : 1u) << 3 * e;
+      for (int j = 0; j < 8; ++j) {
+        const size_t at = ((size_t)__shfl_sync(0xffffffffu, row, i + j) * p.kv_heads + kvh) * kDim + lane * 4;
+        v[j] = *reinterpret_cast<const uint2*>((const T*)p.v_cache + at);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float2 a = Cvt<T>::up(v[j].x), b = Cvt<T>::up(v[j].y);
+        const float f[4] = {a.x, a.y, b.x, b.y};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) seen |= (f[e] == INFINITY ? 2u : f[e] == -INFINITY ? 4u : f[e] == f[e] ? 0u : 1u) << 3 * e;
+      }
     }
   }
   return seen;
