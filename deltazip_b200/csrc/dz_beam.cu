@@ -17,9 +17,8 @@
 // before, 58 with it, as both were then).  Measured from a cold cache: 284 rows of 131072 tokens in bf16, groups of up to 16,
 // k = 32 (74 MB, 11.4 us at the copy bandwidth): 48 us, of which the profiler gives the second launch 13; in the first, issue
 // slots are busy 67 % of the time that an SM has work, the special function unit 26 % and DRAM 25 %, and spans of nine and of
-// seven pieces leave some SMs idle.  128 rows of 32000 floats, k = 16: 24 us; 4 rows, k = 8: 15 to 17.  Not measured: masks
-// that leave fewer than k logits above -inf, where every piece goes the way of naming the best k times.
-// (The first with that as the only way: 180 us in a row of calls, where it takes 42.)
+// seven pieces leave some SMs idle.  128 rows of 32000 floats, k = 16: 21 to 24 us; 4 rows, k = 8: 15 to 17.  Where a mask
+// leaves fewer than k logits above -inf every piece goes the way of naming the best k times: with 5 tokens left 707 and 63 us.
 // Sums are 32-bit within a thread's piece (at most 32 terms) and 64-bit beyond, and so are the scores that rows are compared by:
 // beams come close to one another, and which is ahead is not to hang on a rounding.
 #include "dz_elem.cuh"

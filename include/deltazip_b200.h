@@ -556,10 +556,10 @@ int dz_moe_gemm(const void* x, const void* weights, const int32_t* offsets, cons
  *   beam_select   logits z [rows, vocab] (dtype, rows row_stride elements apart), scores c [rows]; group g holds
  *                 rows group_starts[g] <= r < group_starts[g + 1] (rising) and gets the k best continuations by
  *                 c[r] + z[r, v] - log sum_v exp z[r, v], best first, ties to the lower row, then the lower token.
- *                 NaN logits count as -inf; logits of +inf share the whole probability of their row (the order of
- *                 the others is not said); rows without a logit above -inf or with a score that is not finite have
- *                 scores of -inf alone.  Places without a candidate: score -inf, row and token -1.  k <= 128,
- *                 rows <= 65535.  The workspace needs no preparation.
+ *                 Zeros of both signs are equal.  NaN logits count as -inf; logits of +inf share the whole probability
+ *                 of their row (the order of the others is not said); rows without a logit above -inf or with a score
+ *                 that is not finite have scores of -inf alone.  Places without a candidate: score -inf, row and token
+ *                 -1.  k <= 128, rows <= 65535.  The workspace needs no preparation.
  *   copy_pages    pools: a device table of num_pools entries {address, bytes of a row, rows of a page, bytes of a unit},
  *                 a unit being the largest power of two up to 16 that divides address and row bytes; a pool is num_pages
  *                 pages of page_rows rows.  For pairs (src, dst, rows) the first rows (NULL: all) of page dst become
@@ -573,8 +573,10 @@ int dz_moe_gemm(const void* x, const void* weights, const int32_t* offsets, cons
  *                 tables begin alike), which are read once for the first max_group of them.  A sequence shorter than
  *                 that, or outside the groups, is read by itself; shared lengths above max_shared are read as
  *                 max_shared.  1 to 16 query heads per kv head.  A page number outside the cache is read as its
- *                 last rows.  At most dz_shared_attention_max_seqs() sequences and groups.  The workspace (dz_shared_attention_workspace_bytes, max_keys = table_width *
- *                 block_size) needs no preparation.
+ *                 last rows.  An infinity among the values gives that infinity, however small its weight.  At most
+ *                 dz_shared_attention_max_seqs() sequences and groups.  The workspace (dz_shared_attention_workspace_bytes,
+ *                 max_keys = table_width * block_size) needs no preparation; it is 520 bytes for each of up to 64 parts of
+ *                 a sequence's query head: max_keys / 32 + 3 parts.
  */
 size_t dz_beam_select_workspace_bytes(int rows, int vocab, int k);
 int dz_beam_select(const void* logits, int64_t row_stride, int rows, int vocab, const float* scores, const int32_t* group_starts,
