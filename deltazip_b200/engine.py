@@ -421,7 +421,7 @@ class DecodeEngine:
             raise RuntimeError("sequences are already running")
         if max_new < 1 or any(not p for p in prompts):
             raise ValueError("prompts hold at least a token, and at least one token is generated")
-        if not self.model.whole_vocabulary:
+        if not getattr(self.model, "whole_vocabulary", True):
             raise ValueError("a beam search needs the whole vocabulary on one rank")
         if not 1 <= beams <= min(self.max_seqs, 64):
             raise ValueError(f"between 1 and {min(self.max_seqs, 64)} hypotheses a prompt")
